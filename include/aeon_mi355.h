@@ -406,6 +406,76 @@ int aeon_moe_layer_decode_noalloc(const aeon_moe_layer* layer, const void* d_x, 
 const float* aeon_moe_layer_logits(const aeon_moe_layer* layer, int tokens, void* d_workspace);
 
 /* ------------------------------------------------------------------------------------------
+ * Dense and expert products over unquantised fp16 or bf16 weights
+ * ---------------------------------------------------------------------------------------- */
+
+#define AEON_DTYPE_F16 0
+#define AEON_DTYPE_BF16 1
+
+#define AEON_ACT_NONE 0
+#define AEON_ACT_SILU 1      /* g / (1 + exp(-g)) */
+#define AEON_ACT_GELU 2      /* g/2 * (1 + erf(g / sqrt 2)) */
+#define AEON_ACT_GELU_TANH 3 /* g/2 * (1 + tanh(sqrt(2/pi) * (g + 0.044715 g^3))) */
+#define AEON_ACT_SWIGLU 4    /* silu(min(g, L)) * clamp(u, -L, L) of two matrices; NaN stays NaN */
+
+/* One weight matrix (two for the gated activation), or one per expert, and what follows the
+ * product. Every 16-bit operand of a call (activations, weights, biases, residual, output) is of
+ * `dtype`; products and sums are fp32, and the result is rounded once. Any in_dim, out_dim and
+ * pitch is taken; bases on 16-byte boundaries and pitches that are multiples of 8 elements run
+ * the faster kernels. */
+typedef struct {
+    int dtype;
+    int in_dim;
+    int out_dim;
+    int activation;
+    const void* d_weight;    /* [out_dim][in_dim], row pitch weight_stride elements */
+    const void* d_weight_up; /* AEON_ACT_SWIGLU: the second matrix, same shape and pitches; else NULL */
+    long weight_stride;
+    const void* d_bias;      /* [out_dim] ([experts][out_dim]), nullable */
+    const void* d_bias_up;   /* the second matrix's, nullable */
+    float swiglu_limit;      /* AEON_ACT_SWIGLU: L > 0, INFINITY for no clamp */
+} aeon_projection;
+
+/* y[t][o] = round(act(sum_i x[t][i] * W[o][i] + bias[o]) + residual[t][o]) for `tokens` rows, from
+ * one token to a long prefill. d_residual is nullable and may be d_y (same pitch); d_y must overlap
+ * nothing else. The sum of an output is taken in a fixed order, so a run is reproducible. Few rows
+ * are cut along in_dim, and the shares meet in the workspace (16-byte boundary; 0 bytes where
+ * nothing is cut). The workspace is only used inside the call's own launches. */
+size_t aeon_linear_workspace_bytes(const aeon_projection* projection, int tokens);
+int aeon_linear(const aeon_projection* projection, const void* d_x, long x_stride, int tokens,
+                const void* d_residual, long residual_stride, void* d_y, long y_stride,
+                void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The same product by expert over ragged lists, the unquantised counterpart of
+ * dispatch_aeon_moe_grouped_w13_swiglu_wmma (src/architecture/deepseek_v4/kernels/
+ * moe_grouped_dispatch.hpp:45-64) for any number of experts (<= 1024) in one launch: expert e's
+ * matrices start expert_stride elements after expert e-1's, and positions expert_offsets[e] ..
+ * expert_offsets[e+1]-1 are its list (aeon_expert_permutation), so that
+ * y[p] = round(act(W_e x[row_indices[p]] + bias_e)); without row_indices row p itself. d_x has x_rows
+ * rows. Rows of y behind the last list, and those of a position whose row index is outside
+ * [0, x_rows), are left as they were. An expert without positions is not read. */
+int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,
+                       const void* d_x, long x_stride, int x_rows, const int32_t* d_expert_offsets,
+                       const int32_t* d_row_indices, int positions, void* d_y, long y_stride,
+                       void* stream);
+
+/* The down projection and the way back to tokens, the unquantised counterpart of
+ * dispatch_aeon_moe_grouped_w2_wmma + the fixed-order reduce (moe_grouped_dispatch.hpp:66-88,
+ * src/architecture/deepseek_v4/moe/moe_grouped_batch.hpp:119-146):
+ * out[t] = round(base[t] + sum over s ascending of weights[t][s] * (W_e h[p] + bias_e)), where p is the
+ * position whose draw_indices[p] is t*slots + s, and e = ids[t][s] the expert that lists it. The
+ * contributions stay fp32 (workspace, tokens * slots * out_dim floats). A slot whose id is outside
+ * [0, experts) contributes nothing. d_base is nullable and may be d_out (same pitch). The projection
+ * has no activation. d_h has tokens * slots rows, by position. */
+size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots);
+int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,
+                        const void* d_h, long h_stride, const int32_t* d_expert_offsets,
+                        const int32_t* d_draw_indices, const int32_t* d_topk_ids,
+                        const float* d_topk_weights, int tokens, int slots, const void* d_base,
+                        long base_stride, void* d_out, long out_stride, void* d_workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Hyper-connection stream mix (hc_mult = 4)
  * ---------------------------------------------------------------------------------------- */
 

@@ -70,6 +70,8 @@ def lib():
         _lib.aeon_moe_layer_workspace_bytes.restype = C.c_size_t
         _lib.aeon_router_logits_workspace_bytes.restype = C.c_size_t
         _lib.aeon_a64_slot_bytes.restype = C.c_size_t
+        _lib.aeon_linear_workspace_bytes.restype = C.c_size_t
+        _lib.aeon_expert_combine_workspace_bytes.restype = C.c_size_t
         _lib.aeon_expert_catalog_close.restype = None
     return _lib
 

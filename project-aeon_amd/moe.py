@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import capi, synth
+from . import capi, dense, synth
 
 CFG13 = (4, 8)
 CFG2 = (8, 4)
@@ -232,6 +232,66 @@ class MoeLayer:
                   capi.vp(out), tokens, self.cfg.hidden, E, capi.vp(ws), C.c_size_t(ws.numel()),
                   stream_ptr())
         return out
+
+
+class UnquantisedMoeLayer:
+    """MoeLayer over experts that are not quantised: w1, w3 [experts][intermediate][hidden] and w2
+    [experts][hidden][intermediate] of one type, fp16 or bf16, which is the activations' too. The same
+    router, permutation and roundings (hidden rows in that type, contributions fp32, slots in order), for
+    one token as for a prefill chunk. `dense_shared`: (w1, w3, w2) of an always-on expert, its output
+    the value the routed sum starts from. The router is MoeLayer's for fp16 activations; for bf16 the gate
+    is router_weight_16, bf16 [experts][hidden], with logits rounded to bf16."""
+
+    def __init__(self, w1, w3, w2, top_k, swiglu_limit, router_weight=None, router_bias=None, score_kind=1,
+                 routed_scaling_factor=1.0, renormalize=True, router_weight_16=None, dense_shared=None):
+        experts, inter, hidden = w1.shape
+        if tuple(w3.shape) != (experts, inter, hidden) or tuple(w2.shape) != (experts, hidden, inter):
+            raise ValueError("w1, w3 have to be [experts][intermediate][hidden] and w2 [experts][hidden][intermediate]")
+        if router_weight is not None and w1.dtype != torch.float16:
+            raise ValueError("the fp32 gate takes fp16 activations; give router_weight_16")
+        self.w1, self.w3, self.w2 = w1, w3, w2
+        self.router_weight, self.router_weight_16, self.router_bias = router_weight, router_weight_16, router_bias
+        self.dense_shared = dense_shared
+        self.cfg = MoeLayerStruct(hidden, inter, experts, top_k, 0, swiglu_limit, score_kind, routed_scaling_factor,
+                                  int(renormalize))
+
+    def router_logits(self, x):
+        """fp32 logits [tokens][experts] of x."""
+        experts, hidden = self.cfg.experts, self.cfg.hidden
+        if self.router_weight is None:
+            return dense.linear(x, self.router_weight_16).float()
+        out = torch.empty(x.shape[0], experts, dtype=torch.float32, device=x.device)
+        n = capi.lib().aeon_router_logits_workspace_bytes(x.shape[0], hidden, experts)
+        ws = torch.empty(max(n, 4), dtype=torch.uint8, device=x.device)
+        capi.call("aeon_router_logits", capi.vp(x), x.stride(0), capi.vp(self.router_weight), capi.vp(out),
+                  x.shape[0], hidden, experts, capi.vp(ws), C.c_size_t(ws.numel()), stream_ptr())
+        return out
+
+    def decode(self, x, out=None, ids=None, weights=None):
+        """x [tokens][hidden] -> (out [tokens][hidden], ids int32, weights fp32), MoeLayer.decode's contract."""
+        tokens, k = x.shape[0], self.cfg.top_k
+        ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device) if ids is None else ids
+        weights = (torch.empty(tokens, k, dtype=torch.float32, device=x.device)
+                   if weights is None else weights)
+        logits = self.router_logits(x)
+        capi.call("aeon_moe_router", capi.vp(logits), capi.vp(self.router_bias), None, None, capi.vp(weights),
+                  capi.vp(ids), tokens, self.cfg.experts, k, C.c_float(self.cfg.routed_scaling_factor),
+                  self.cfg.renormalize, self.cfg.score_kind, stream_ptr())
+        return self.routed(x, ids, weights, out), ids, weights
+
+    def routed(self, x, ids, weights, out=None):
+        """The expert part for given routing. Without an always-on expert the routed sum is added to what
+        `out` holds (an `out` allocated here starts from zero), as MoeLayer.routed does."""
+        limit = self.cfg.swiglu_limit
+        base = out
+        if self.dense_shared is not None:
+            w1, w3, w2 = self.dense_shared
+            h = dense.linear(x, w1, weight_up=w3, activation="swiglu", swiglu_limit=limit)
+            base = out = dense.linear(h, w2, out=out)
+        lists = dense.expert_lists(ids, self.cfg.experts)
+        h = dense.expert_linear(x, self.w1, lists.offsets, lists.rows, weight_up=self.w3, activation="swiglu",
+                                swiglu_limit=limit)
+        return dense.expert_combine(h, self.w2, lists.offsets, lists.draws, ids, weights, base=base, out=out)
 
 
 class HyperConnection:

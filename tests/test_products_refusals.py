@@ -1,0 +1,119 @@
+"""What the entry points of the unquantised products refuse, before any device work."""
+import ctypes as C
+
+import pytest
+
+from project_aeon_amd import capi, dense
+
+A = C.c_void_p(1 << 20)        # never dereferenced: every call below is refused first, or has nothing to do
+B = C.c_void_p(1 << 21)
+ODD = C.c_void_p((1 << 20) + 1)
+
+
+def _p(**change):
+    fields = dict(dtype=0, in_dim=64, out_dim=32, activation=0, d_weight=1 << 22, d_weight_up=None, weight_stride=64,
+                  d_bias=None, d_bias_up=None, swiglu_limit=0.0)
+    fields.update(change)
+    return dense.Projection(**fields)
+
+
+def _linear(p, x=A, xs=64, tokens=4, res=None, rs=0, y=B, ys=32, ws=None, wb=0):
+    capi.call("aeon_linear", None if p is None else C.byref(p), x, C.c_long(xs), tokens, res, C.c_long(rs), y, C.c_long(ys),
+              ws, C.c_size_t(wb), None)
+
+
+def _experts(p, experts=4, es=2048, x=A, xs=64, x_rows=8, off=A, rows=None, positions=8, y=B, ys=32):
+    capi.call("aeon_expert_linear", C.byref(p), experts, C.c_long(es), x, C.c_long(xs), x_rows, off, rows, positions, y,
+              C.c_long(ys), None)
+
+
+def _combine(p, experts=4, es=2048, h=A, hs=64, off=A, draws=A, ids=A, w=A, tokens=4, slots=2, base=None, bs=0, out=B,
+             os=32, ws=A, wb=1 << 30):
+    capi.call("aeon_expert_combine", C.byref(p), experts, C.c_long(es), h, C.c_long(hs), off, draws, ids, w, tokens, slots,
+              base, C.c_long(bs), out, C.c_long(os), ws, C.c_size_t(wb), None)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), "unknown dtype"), (dict(dtype=-1), "unknown dtype"),
+    (dict(in_dim=0), "bad shape"), (dict(out_dim=-3), "bad shape"), (dict(in_dim=1 << 25, weight_stride=1 << 25), "bad shape"),
+    (dict(weight_stride=63), "overlap"), (dict(activation=5), "unknown activation"), (dict(activation=-1), "unknown activation"),
+    (dict(d_weight=None), "null weight"), (dict(activation=4, swiglu_limit=7.0), "second weight matrix"),
+    (dict(d_weight_up=1 << 23), "second weight matrix"), (dict(d_bias_up=1 << 23), "second bias"),
+    (dict(activation=4, d_weight_up=1 << 23), "swiglu_limit"),
+    (dict(activation=4, d_weight_up=1 << 23, swiglu_limit=float("nan")), "swiglu_limit"),
+    (dict(d_weight=(1 << 22) + 1), "odd address"), (dict(d_bias=(1 << 22) + 1), "odd address")])
+def test_projection_refusals(change, text):
+    for call in (_linear, _experts, _combine):
+        with pytest.raises(ValueError, match=text):
+            call(_p(**change))
+    assert capi.lib().aeon_linear_workspace_bytes(C.byref(_p(**change)), 4) == 0
+    assert capi.lib().aeon_expert_combine_workspace_bytes(C.byref(_p(**change)), 4, 2) == 0
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(tokens=-1), "negative"), (dict(x=None), "null buffer"), (dict(y=None), "null buffer"), (dict(x=ODD), "odd address"),
+    (dict(y=ODD), "odd address"), (dict(res=ODD, rs=32), "odd address"), (dict(xs=63), "row pitch"), (dict(ys=31), "row pitch"),
+    (dict(res=A, rs=31), "row pitch"), (dict(y=A), "must not alias"), (dict(y=C.c_void_p(1 << 22)), "must not alias"),
+    (dict(res=B, rs=40), "residual's row pitch")])
+def test_linear_refusals(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _linear(_p(), **kw)
+
+
+def test_linear_refuses_a_short_workspace():
+    p = _p(in_dim=7168, weight_stride=7168, out_dim=256)
+    need = capi.lib().aeon_linear_workspace_bytes(C.byref(p), 1)
+    assert need > 0 and need % (256 * 4) == 0
+    for ws, wb in ((None, need), (A, need - 1), (C.c_void_p((1 << 20) + 4), need)):
+        with pytest.raises(ValueError, match="workspace of"):
+            _linear(p, xs=7168, ys=256, tokens=1, ws=ws, wb=wb)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(experts=0), "expert count"), (dict(experts=1025), "expert count"), (dict(es=2047), "overlap"),
+    (dict(positions=-1), "negative"), (dict(x=None), "null buffer"), (dict(off=None), "null buffer"),
+    (dict(y=None), "null buffer"), (dict(x_rows=7), "7 rows for 8"), (dict(x_rows=0, rows=A), "0 rows"),
+    (dict(x=ODD), "boundary"), (dict(off=C.c_void_p((1 << 20) + 2)), "boundary"), (dict(xs=8), "row pitch"),
+    (dict(ys=8), "row pitch"), (dict(y=A), "must not alias")])
+def test_expert_linear_refusals(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _experts(_p(), **kw)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(experts=2000), "expert count"), (dict(es=100), "overlap"), (dict(tokens=-1), "bad draw shape"),
+    (dict(slots=0), "bad draw shape"), (dict(tokens=1 << 30, slots=4), "bad draw shape"), (dict(h=None), "null buffer"),
+    (dict(draws=None), "null buffer"), (dict(ids=None), "null buffer"), (dict(w=None), "null buffer"),
+    (dict(out=None), "null buffer"), (dict(h=ODD), "boundary"), (dict(w=C.c_void_p(2)), "boundary"), (dict(hs=1), "row pitch"),
+    (dict(os=1), "row pitch"), (dict(base=A, bs=1), "row pitch"), (dict(out=A), "must not alias"),
+    (dict(base=B, bs=40), "base's row pitch"), (dict(ws=None), "workspace of"), (dict(wb=8), "workspace of")])
+def test_expert_combine_refusals(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _combine(_p(), **kw)
+
+
+def test_combine_takes_no_activation():
+    with pytest.raises(ValueError, match="no activation"):
+        _combine(_p(activation=1))
+
+
+def test_null_projection_and_calls_with_nothing_to_do():
+    with pytest.raises(ValueError, match="null projection"):
+        _linear(None)
+    _linear(_p(), tokens=0, x=None, y=None)
+    _experts(_p(), positions=0, x=None, y=None)
+    _combine(_p(), tokens=0, h=None, out=None)
+
+
+def test_the_tensor_functions_check_their_operands():
+    import torch
+    x, w = torch.zeros(2, 8, dtype=torch.float16), torch.zeros(4, 8, dtype=torch.float16)
+    with pytest.raises(ValueError, match="on a GPU"):
+        dense.linear(x, w)
+    with pytest.raises(ValueError, match="on a GPU"):
+        dense.linear(x.double(), w)
+    with pytest.raises(ValueError, match="on a GPU"):
+        dense.expert_lists(torch.zeros(2, 2, dtype=torch.int32), 4)
+    with pytest.raises(ValueError, match="hidden"):
+        from project_aeon_amd import moe
+        moe.UnquantisedMoeLayer(torch.zeros(2, 3, 4), torch.zeros(2, 3, 4), torch.zeros(2, 3, 4), 1, 7.0)
