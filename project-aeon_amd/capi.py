@@ -70,8 +70,16 @@ def lib():
         _lib.aeon_moe_layer_workspace_bytes.restype = C.c_size_t
         _lib.aeon_router_logits_workspace_bytes.restype = C.c_size_t
         _lib.aeon_a64_slot_bytes.restype = C.c_size_t
-        _lib.aeon_linear_workspace_bytes.restype = C.c_size_t
-        _lib.aeon_expert_combine_workspace_bytes.restype = C.c_size_t
+        # declared in full: callers pass plain numbers, which costs less per call than wrapping each
+        p, n, i = C.c_void_p, C.c_long, C.c_int
+        for name, result, args in (
+                ("aeon_linear_workspace_bytes", C.c_size_t, (p, i)),
+                ("aeon_linear", i, (p, p, n, i, p, n, p, n, p, C.c_size_t, p)),
+                ("aeon_expert_linear", i, (p, i, n, p, n, i, p, p, i, p, n, p)),
+                ("aeon_expert_combine_workspace_bytes", C.c_size_t, (p, i, i)),
+                ("aeon_expert_combine", i, (p, i, n, p, n, p, p, p, p, i, i, p, n, p, n, p, C.c_size_t, p))):
+            entry = getattr(_lib, name)
+            entry.restype, entry.argtypes = result, args
         _lib.aeon_expert_catalog_close.restype = None
     return _lib
 

@@ -19,15 +19,20 @@
 #include "product.hpp"
 
 #include <atomic>
+#include <type_traits>
 
 namespace aeon355 {
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
+template <int N>
+using C = std::integral_constant<int, N>;
+
 constexpr int kStep = 64;           // columns of one pipeline step: 128 bytes of a row
 constexpr int kStepBytes = 128;
 constexpr int kXcds = 8;
+constexpr int kXcdCus = 32;
 constexpr int kWindowGroup = 8;     // windows that share a pass over the row blocks
 
 struct F16 {
@@ -75,14 +80,22 @@ __device__ __forceinline__ float activate(int kind, float g, float u, float limi
 // It has no register result, so nothing is in flight that the compiler could reuse; the waits are
 // wait_requests() before the barrier that publishes a stage. M0 is never live across instructions the
 // compiler emits: it writes it right before each use.
+// STREAM: the bytes are read by this workgroup alone and should not push others out of the caches.
+template <bool STREAM>
 __device__ __forceinline__ void request_to_lds(const char* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :: "s"(lds), "v"(p) : "memory");
+    if constexpr (STREAM) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
+    } else {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
+    }
 }
 template <int N>
 __device__ __forceinline__ void wait_requests() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "i"(N) : "memory");
 }
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void bare_barrier() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -90,13 +103,17 @@ __device__ __forceinline__ void bare_barrier() {
 
 struct ProductTile {
     int expert, first, count, row_block;  // positions [first, first + count), row block of W
+    bool only;                            // no other window of the list reads these rows
 };
 
 // Tile of workgroup b. Workgroups are dealt to the 8 XCDs round robin, so tile numbers are handed
 // out in 8 contiguous runs, one per XCD: neighbouring tiles share panels through one L2. Inside an
 // expert up to kWindowGroup windows take turns over each row block, a near-square patch of the
 // output for the workgroups that run at the same time.
-template <int BM>
+// HALVES: one workgroup fills a CU, and a tile may be run as two of half the positions at half the
+// cost each. Where at most half of the CUs would have a tile in an XCD's last round, the tiles of that
+// round are cut so.
+template <int BM, bool HALVES>
 __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, int b, ProductTile* t) {
     const int lane = threadIdx.x & 63;
     int expert = 0, first = 0, held = a.positions, before = 0, windows;
@@ -133,7 +150,14 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
         total = __builtin_amdgcn_readlane(upto, 63) * row_blocks;
     }
     const int run = (total + kXcds - 1) / kXcds;
-    const int at = b / kXcds;
+    int at = b / kXcds, half = -1;
+    if (HALVES) {
+        const int last = run % kXcdCus;
+        if (last <= kXcdCus / 2 && at >= run - last) {
+            half = (at - (run - last)) & 1;
+            at = run - last + (at - (run - last)) / 2;
+        }
+    }
     const int tile = (b % kXcds) * run + at;
     if (at >= run || tile >= total) return false;
     if (a.offsets != nullptr) {
@@ -166,23 +190,71 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
     const int window = group * kWindowGroup + v % wide;
     t->expert = expert;
     t->row_block = v / wide;
+    t->only = windows == 1;
     t->first = first + window * BM;
     const int rest = held - window * BM;
     t->count = rest < BM ? rest : BM;
-    return true;
+    if (HALVES && half >= 0) {
+        t->first += half * (BM / 2);
+        t->count -= half * (BM / 2);
+        if (half == 0 && t->count > BM / 2) t->count = BM / 2;
+    }
+    return t->count > 0;
 }
 
-// 16 bytes of a row starting at column c, zeros from column k on. `p` is the row's column 0. The
-// address may be off every boundary but the element's; loads of global memory take that.
+// 16 bytes of a row starting at column c, zeros from column k on. `p` is the row's column 0; nothing
+// outside the row's k columns is read. The address may be off every boundary but the element's; loads of
+// global memory take that.
 __device__ __forceinline__ u32x4_t load_columns(const uint16_t* p, int c, int k) {
     typedef u32x4_t __attribute__((aligned(2))) loose_t;
-    if (c + 8 <= k) return *reinterpret_cast<const loose_t*>(p + c);
-    u32x4_t v = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (c + i < k) v[i / 2] |= static_cast<uint32_t>(p[c + i]) << (16 * (i & 1));
+    const AEON_GLOBAL uint16_t* row = as_global<uint16_t>(p);
+    if (c + 8 <= k) return *reinterpret_cast<const AEON_GLOBAL loose_t*>(row + c);
+    unsigned __int128 v = 0;
+    if (c < k && k >= 8) {  // the row's last eight values, the ones before column c shifted out
+        v = __builtin_bit_cast(unsigned __int128, *reinterpret_cast<const AEON_GLOBAL loose_t*>(row + k - 8));
+        v >>= (c + 8 - k) * 16;
+    } else {
+#pragma unroll 1
+        for (int i = k - 1; i >= c; --i) v = v << 16 | row[i];
     }
-    return v;
+    return __builtin_bit_cast(u32x4_t, v);
+}
+
+__device__ __forceinline__ void store_wide(float* dst, const float4_t& v, int o, int n) {
+    if (n % 4 == 0) {
+        *reinterpret_cast<float4_t*>(dst) = v;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (o + q < n) dst[q] = v[q];
+    }
+}
+
+// The residual and the one rounding, outputs o .. o + 3 of position p.
+template <class T>
+__device__ __forceinline__ void finish(const ProductArgs& a, int p, int o, float4_t g) {
+    uint16_t* dst = a.y + p * a.y_stride + o;
+    const uint16_t* res = a.residual == nullptr ? nullptr : a.residual + p * a.residual_stride + o;
+    if (a.vec_out) {
+        if (res != nullptr) {
+            const uint2 r = *reinterpret_cast<const uint2*>(res);
+            g[0] += T::widen(r.x & 0xFFFFu);
+            g[1] += T::widen(r.x >> 16);
+            g[2] += T::widen(r.y & 0xFFFFu);
+            g[3] += T::widen(r.y >> 16);
+        }
+        uint2 v;
+        v.x = T::round(g[0]) | (static_cast<uint32_t>(T::round(g[1])) << 16);
+        v.y = T::round(g[2]) | (static_cast<uint32_t>(T::round(g[3])) << 16);
+        *reinterpret_cast<uint2*>(dst) = v;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (o + q >= a.n) break;
+            if (res != nullptr) g[q] += T::widen(res[q]);
+            dst[q] = T::round(g[q]);
+        }
+    }
 }
 
 // ALIGNED: x and W start on 16-byte boundaries and their pitches are multiples of 8 elements.
@@ -192,9 +264,11 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     constexpr int WAVES = WAVES_M * WAVES_N;
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
     constexpr int TM = WM / 16, TN = WN / 16;
-    constexpr int NI = (BM + BN) / 8 / WAVES;  // requests of a wave per step
+    constexpr int NW = BN / 8 / WAVES, NI = NW + BM / 8 / WAVES;  // requests of a wave per step: weights, then positions
     constexpr int STAGE = (BM + BN) * kStepBytes;
-    static_assert((BM + BN) / 8 % WAVES == 0 && TN % 2 == 0 && BM % 16 == 0 && (ALIGNED || S == 2), "tile");
+    constexpr bool TURNS = ALIGNED && BM == 256 && BN == 256;
+    static_assert(!TURNS || (WAVES == 8 && S == 2 && TM == 8 && TN == 4), "the schedule of the waves that take turns");
+    static_assert(BN / 8 % WAVES == 0 && BM / 8 % WAVES == 0 && TN % 2 == 0 && BM % 16 == 0 && (ALIGNED || S == 2), "tile");
     extern __shared__ char ring[];
 
     const int lane = threadIdx.x & 63;
@@ -203,7 +277,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     const int rows_per_block = a.pair ? BN / 2 : BN;
     const int row_blocks = (a.n + rows_per_block - 1) / rows_per_block;
     ProductTile t;
-    if (!find_tile<BM>(a, row_blocks, blockIdx.x, &t)) return;
+    if (!find_tile<BM, TURNS>(a, row_blocks, blockIdx.x, &t)) return;
     const int n0 = t.row_block * rows_per_block;
 
     int step0 = 0, steps = (a.k + kStep - 1) / kStep;
@@ -212,13 +286,31 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         steps = steps - step0 < a.split_steps ? steps - step0 : a.split_steps;
     }
 
+    // First panel row of a wave's request i. The kernel whose waves take turns asks for a step in
+    // four parts, two requests a wave each: the first half of every wave's weight rows, the first
+    // half of its positions, and the second halves.
+    auto panel_row = [&](int i) __attribute__((always_inline)) {
+        if constexpr (TURNS) {
+            const int q = (wave * 2 + (i & 1)) * 8;
+            const int half = i / 4;
+            return (i / 2) % 2 == 0 ? q / (WN / 2) * WN + half * (WN / 2) + q % (WN / 2)
+                                    : BN + q / (WM / 2) * WM + half * (WM / 2) + q % (WM / 2);
+        } else {
+            return i < NW ? (wave * NW + i) * 8 : BN + (wave * (NI - NW) + i - NW) * 8;
+        }
+    };
+    // Position a panel row holds. Where waves take turns, a wave's first half of positions lies in the
+    // tile's first half: a tile with no more than that many live ones skips the second halves.
+    auto position_of = [&](int r) __attribute__((always_inline)) {
+        return TURNS ? r % WM / (WM / 2) * (BM / 2) + r / WM * (WM / 2) + r % (WM / 2) : r;
+    };
     // this lane's row of every request: panel rows [0, BN) are weights, [BN, BN + BM) positions;
     // rows past the end repeat the last one and are not stored
     const uint16_t* src[NI];
     const int unit = (lane & 7) ^ (lane >> 3);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-        const int r = (wave * NI + i) * 8 + (lane >> 3);
+        const int r = panel_row(i) + (lane >> 3);
         if (r < BN) {
             int matrix = 0, row = r;
             if (a.pair) {
@@ -230,7 +322,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             row = row < a.n ? row : a.n - 1;
             src[i] = a.w[matrix] + t.expert * a.expert_stride + row * a.w_stride;
         } else {
-            int m = r - BN;
+            int m = position_of(r - BN);
             m = t.first + (m < t.count ? m : t.count - 1);
             if (a.rows != nullptr) {
                 m = a.rows[m];
@@ -248,37 +340,32 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
 
     const uint32_t ring_at = static_cast<uint32_t>(
         reinterpret_cast<size_t>((__attribute__((address_space(3))) char*)ring));
-    u32x4_t held[ALIGNED ? 1 : NI];
-    auto fetch = [&](int step) {  // a step's share through registers
-#pragma unroll
-        for (int i = 0; i < NI; ++i) held[ALIGNED ? 0 : i] = load_columns(src[i], (step0 + step) * kStep + unit * 8, a.k);
-    };
-    auto put = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            *reinterpret_cast<u32x4_t*>(ring + stage * STAGE + (wave * NI + i) * 1024 + lane * 16) = held[ALIGNED ? 0 : i];
-        }
-    };
     const int whole = (a.k - step0 * kStep) / kStep;
-    const int full = whole < steps ? whole : steps;  // steps before this one have all 64 columns
-    auto request = [&](int step, int stage) {
-        if (step < full) {
+    const int full = whole < steps ? whole : steps;  // steps of 64 columns; a shorter one may follow
+    // requests [first, first + count) of a whole step
+    auto request = [&](int step, int stage, auto first, auto count, auto stream) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                request_to_lds(reinterpret_cast<const char*>(src[i]) + unit * 16 +
-                                   static_cast<size_t>(step0 + step) * kStepBytes,
-                               ring_at + stage * STAGE + (wave * NI + i) * 1024);
-            }
-        } else {  // the last columns of a K that is no multiple of 64
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                *reinterpret_cast<u32x4_t*>(ring + stage * STAGE + (wave * NI + i) * 1024 + lane * 16) =
-                    load_columns(src[i], (step0 + step) * kStep + unit * 8, a.k);
-            }
+        for (int i = first; i < first + count; ++i) {
+            const char* p = reinterpret_cast<const char*>(src[i]) + unit * 16 +
+                            static_cast<size_t>(step0 + step) * kStepBytes;
+            const uint32_t lds = ring_at + stage * STAGE + panel_row(i) * kStepBytes;
+            if (stream && i < NW) request_to_lds<true>(p, lds);
+            else request_to_lds<false>(p, lds);
         }
+    };
+    // a step through registers, columns from K on as zeros
+    u32x4_t held[NI];
+    auto fetch = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) held[i] = load_columns(src[i], (step0 + step) * kStep + unit * 8, a.k);
+    };
+    auto put = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            *reinterpret_cast<u32x4_t*>(ring + stage * STAGE + panel_row(i) * kStepBytes + lane * 16) = held[i];
     };
     const int frag = (lane & 15) * kStepBytes + (((lane >> 4) ^ (lane & 7)) * 16);
-    auto multiply = [&](int stage) {
+    auto multiply = [&](int stage) __attribute__((always_inline)) {
         const char* wp = ring + stage * STAGE + wave_n * WN * kStepBytes;
         const char* xp = ring + stage * STAGE + (BN + wave_m * WM) * kStepBytes;
 #pragma unroll
@@ -295,22 +382,126 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         }
     };
 
-    if constexpr (ALIGNED) {
+    if constexpr (TURNS) {
+        // Two waves share a SIMD; they take turns at its matrix pipe. A step is four quarters of
+        // the wave's tile, and a quarter a fetch part (LDS reads, requests) and a multiply part,
+        // each ended by a barrier; waves 4..7 run one barrier behind waves 0..3, so that one wave
+        // of a SIMD fetches while the other multiplies. A part's LDS reads have landed when its
+        // barrier opens, so the region they came from is asked for again, for two steps later, one
+        // fetch part on; a part waits for what the next one reads. Requests are therefore up to
+        // 14 deep per wave (112 KB of a CU's 128 KB of panels).
+        u32x4_t wf[2][2][2], xf[4][2];  // [half of the weight rows][tile][columns 32h..], [tile][columns]
+        auto read_w = [&](int stage, auto half) __attribute__((always_inline)) {
+            const char* wp = ring + stage * STAGE + (wave_n * WN + half * (WN / 2)) * kStepBytes;
 #pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-            if (s < steps) request(s, s);
-        }
-        int stage = 0, ahead = S - 1;
-        for (int s = 0; s < steps; ++s) {
-            // the S-2 younger steps may still be under way, if they are all requests
-            if (s + S - 2 < full) wait_requests<(S - 2) * NI>();
-            else wait_requests<0>();
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    wf[half][i][h] = *reinterpret_cast<const u32x4_t*>(wp + i * 2048 + (frag ^ (h * 64)));
+        };
+        auto read_x = [&](int stage, auto half) __attribute__((always_inline)) {
+            const char* xp = ring + stage * STAGE + (BN + wave_m * WM + half * (WM / 2)) * kStepBytes;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    xf[j][h] = *reinterpret_cast<const u32x4_t*>(xp + j * 2048 + (frag ^ (h * 64)));
+        };
+        auto quarter = [&](auto wh, auto xh) __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
             bare_barrier();
-            if (s + S - 1 < steps) request(s + S - 1, ahead);
-            multiply(stage);
-            stage = stage + 1 == S ? 0 : stage + 1;
-            ahead = ahead + 1 == S ? 0 : ahead + 1;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[wh * 2 + i][xh * 4 + j] = T::mfma(wf[wh][i][h], xf[j][h], acc[wh * 2 + i][xh * 4 + j]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            bare_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (t.count > BM / 2) {
+            if (full > 0) request(0, 0, C<0>{}, C<8>{}, std::false_type{});
+            if (full > 1) {
+                request(1, 1, C<0>{}, C<8>{}, std::false_type{});
+                wait_requests<12>();
+            } else {
+                wait_requests<0>();
+            }
+            bare_barrier();
+            if (wave >= 4) bare_barrier();
+            for (int s = 0; s < full; ++s) {
+                const int b = s & 1;
+                const bool more = s + 2 < full;
+                read_w(b, C<0>{});
+                read_x(b, C<0>{});
+                if (more) wait_requests<10>();
+                else wait_requests<0>();
+                quarter(C<0>{}, C<0>{});
+                if (more) request(s + 2, b, C<0>{}, C<4>{}, std::false_type{});
+                read_w(b, C<1>{});
+                if (more) wait_requests<12>();
+                else wait_requests<0>();
+                quarter(C<1>{}, C<0>{});
+                if (more) request(s + 2, b, C<4>{}, C<2>{}, std::false_type{});
+                read_x(b, C<1>{});
+                wait_reads();
+                quarter(C<1>{}, C<1>{});
+                if (more) request(s + 2, b, C<6>{}, C<2>{}, std::false_type{});
+                if (more) wait_requests<12>();
+                else wait_requests<0>();
+                quarter(C<0>{}, C<1>{});
+            }
+        } else {
+            // no second half of positions: two quarters and six requests a step
+            if (full > 0) request(0, 0, C<0>{}, C<6>{}, std::false_type{});
+            if (full > 1) {
+                request(1, 1, C<0>{}, C<4>{}, std::false_type{});
+                wait_requests<6>();
+            } else {
+                wait_requests<0>();
+            }
+            bare_barrier();
+            if (wave >= 4) bare_barrier();
+            for (int s = 0; s < full; ++s) {
+                const int b = s & 1;
+                if (s + 1 < full) request(s + 1, b ^ 1, C<4>{}, C<2>{}, std::false_type{});
+                read_w(b, C<0>{});
+                read_x(b, C<0>{});
+                if (s + 1 < full) wait_requests<6>();
+                else wait_requests<0>();
+                quarter(C<0>{}, C<0>{});
+                if (s + 2 < full) request(s + 2, b, C<0>{}, C<4>{}, std::false_type{});
+                read_w(b, C<1>{});
+                if (s + 2 < full) wait_requests<6>();
+                else wait_requests<0>();
+                quarter(C<1>{}, C<0>{});
+            }
         }
+        if (wave < 4) bare_barrier();
+    } else if constexpr (ALIGNED) {
+        auto ring_loop = [&](auto stream) __attribute__((always_inline)) {
+#pragma unroll
+            for (int s = 0; s < S - 1; ++s) {
+                if (s < full) request(s, s, C<0>{}, C<NI>{}, stream);
+            }
+            int stage = 0, ahead = S - 1;
+            for (int s = 0; s < full; ++s) {
+                if (s + S - 2 < full) wait_requests<(S - 2) * NI>();  // the S-2 younger steps may be under way
+                else wait_requests<0>();
+                bare_barrier();
+                if (s + S - 1 < full) request(s + S - 1, ahead, C<0>{}, C<NI>{}, stream);
+                multiply(stage);
+                stage = stage + 1 == S ? 0 : stage + 1;
+                ahead = ahead + 1 == S ? 0 : ahead + 1;
+            }
+        };
+        if (t.only) ring_loop(std::true_type{});
+        else ring_loop(std::false_type{});
     } else {
         if (steps > 0) {
             fetch(0);
@@ -323,95 +514,330 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             if (s + 1 < steps) put((s + 1) & 1);
         }
     }
+    if (ALIGNED && steps > full) {  // the last columns of a K that is no multiple of 64
+        fetch(full);
+        wait_reads();
+        bare_barrier();
+        put(0);
+        wait_reads();
+        bare_barrier();
+        multiply(0);
+    }
 
-    // Epilogue: lane holds outputs 4*(lane/16) .. +3 of a 16-row tile for position lane%16.
-    const int out0 = n0 + wave_n * (a.pair ? WN / 2 : WN) + (lane >> 4) * 4;
-    const int tiles = a.pair ? TN / 2 : TN;
+    // Epilogue. A lane holds outputs 4*(lane/16) .. +3 of a 16-row tile for position lane%16; the tile
+    // turns through LDS (the ring is done with, every wave has its own share) so that neighbouring
+    // lanes finish and store neighbouring outputs of one position: whole 128-byte lines, and one
+    // copy of the epilogue's code. The 16-byte units of a row are exclusive-ored with the row's
+    // number: neither side meets a bank twice.
+    constexpr int UNITS = WN / 4;  // of a position's row, gate and up together
+    constexpr int SHARE = S * STAGE / WAVES;
+    constexpr int CHUNK = WM * WN * 4 <= SHARE ? WM : WM / 2;  // positions turned at a time
+    static_assert(CHUNK * WN * 4 <= SHARE && CHUNK % 16 == 0 && UNITS <= 16, "the ring holds the turned tile");
+    wait_reads();
+    bare_barrier();
+    float4_t* turned = reinterpret_cast<float4_t*>(ring + wave * SHARE);
+    const int row_units = a.pair ? UNITS / 2 : UNITS;
+    const int turn_u = lane & (row_units - 1);
+    const int turn_rows = 64 / row_units;
+    const int o = n0 + wave_n * (row_units * 4) + turn_u * 4;
+    const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    // the biases of a lane's four outputs are the same for every position
+    float4_t bias[2] = {zero, zero};
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-        const int m = wave_m * WM + j * 16 + (lane & 15);
-        if (m >= t.count) continue;
-        const int p = t.first + m;
-        if (a.rows != nullptr) {
-            const int row = a.rows[p];
-            if (row < 0 || row >= a.x_rows) continue;
-        }
-        long draw = 0;
-        float draw_weight = 0.0f;
-        if (a.mode == kProductDraws) {
-            draw = a.draws[p];
-            if (draw < 0 || draw >= a.draw_count) continue;
-            draw_weight = a.draw_weights[draw];
-        }
+    for (int m = 0; m < 2; ++m) {
+        if (a.bias[m] == nullptr || a.mode == kProductPartial) continue;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-            const int o = out0 + i * 16;
-            if (i >= tiles || o >= a.n) break;
-            float g[4], u[4];
+        for (int q = 0; q < 4; ++q)
+            if (o + q < a.n) bias[m][q] = T::widen(a.bias[m][static_cast<size_t>(t.expert) * a.n + o + q]);
+    }
+#pragma unroll
+    for (int chunk = 0; chunk < WM / CHUNK; ++chunk) {
+#pragma unroll
+        for (int j = 0; j < CHUNK / 16; ++j) {
+            const int r = j * 16 + (lane & 15);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                turned[r * UNITS + ((i * 4 + (lane >> 4)) ^ (r & (UNITS - 1)))] = acc[i][chunk * (CHUNK / 16) + j];
+            }
+        }
+        asm volatile("" ::: "memory");  // LDS serves a wave's accesses in order
+        const int from = position_of(wave_m * WM + chunk * CHUNK);
+        const int live = t.count - from;
+#pragma unroll 1
+        for (int r = lane / row_units; r < CHUNK && r < live; r += turn_rows) {
+            if (o >= a.n) break;
+            const int p = t.first + from + r;
+            float4_t g = turned[r * UNITS + (turn_u ^ (r & (UNITS - 1)))];
+            float4_t u = zero;
+            if (a.pair) u = turned[r * UNITS + ((turn_u + UNITS / 2) ^ (r & (UNITS - 1)))];
             if (a.mode == kProductPartial) {
-#pragma unroll
-                for (int m2 = 0; m2 < 2; ++m2) {
-                    if (m2 == 1 && !a.pair) break;
-                    float* dst = a.wide + ((static_cast<size_t>(blockIdx.y) * (a.pair + 1) + m2) * a.positions + p) * a.n + o;
-                    const float4_t v = m2 == 0 ? acc[i][j] : acc[(i + TN / 2) % TN][j];
-                    if (a.n % 4 == 0) {
-                        *reinterpret_cast<float4_t*>(dst) = v;
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (o + q < a.n) dst[q] = v[q];
-                    }
-                }
+                float* dst = a.wide + (static_cast<size_t>(blockIdx.y) * (a.pair + 1) * a.positions + p) * a.n + o;
+                store_wide(dst, g, o, a.n);
+                if (a.pair) store_wide(dst + static_cast<size_t>(a.positions) * a.n, u, o, a.n);
                 continue;
             }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const bool live = o + q < a.n;
-                g[q] = acc[i][j][q];
-                if (a.bias[0] != nullptr && live) g[q] += T::widen(a.bias[0][static_cast<size_t>(t.expert) * a.n + o + q]);
-                u[q] = 0.0f;
-                if (a.pair) {
-                    u[q] = acc[(i + TN / 2) % TN][j][q];
-                    if (a.bias[1] != nullptr && live) u[q] += T::widen(a.bias[1][static_cast<size_t>(t.expert) * a.n + o + q]);
-                }
-            }
+            g += bias[0];
+            u += bias[1];
             if (a.mode == kProductDraws) {
-                float* dst = a.wide + static_cast<size_t>(draw) * a.n + o;
-                if (a.n % 4 == 0) {
-                    *reinterpret_cast<float4_t*>(dst) = float4_t{g[0], g[1], g[2], g[3]} * draw_weight;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (o + q < a.n) dst[q] = g[q] * draw_weight;
-                }
+                const long draw = a.draws[p];
+                if (draw < 0 || draw >= a.draw_count) continue;
+                store_wide(a.wide + static_cast<size_t>(draw) * a.n + o, g * a.draw_weights[draw], o, a.n);
                 continue;
+            }
+            if (a.rows != nullptr) {
+                const int row = a.rows[p];
+                if (row < 0 || row >= a.x_rows) continue;
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) g[q] = activate(a.activation, g[q], u[q], a.limit);
-            uint16_t* dst = a.y + p * a.y_stride + o;
-            const uint16_t* res = a.residual == nullptr ? nullptr : a.residual + p * a.residual_stride + o;
-            if (a.vec_out) {
-                if (res != nullptr) {
-                    const uint2 r = *reinterpret_cast<const uint2*>(res);
-                    g[0] += T::widen(r.x & 0xFFFFu);
-                    g[1] += T::widen(r.x >> 16);
-                    g[2] += T::widen(r.y & 0xFFFFu);
-                    g[3] += T::widen(r.y >> 16);
-                }
-                uint2 v;
-                v.x = T::round(g[0]) | (static_cast<uint32_t>(T::round(g[1])) << 16);
-                v.y = T::round(g[2]) | (static_cast<uint32_t>(T::round(g[3])) << 16);
-                *reinterpret_cast<uint2*>(dst) = v;
-            } else {
+            finish<T>(a, p, o, g);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// ---- a few positions: one pass of the weights through registers ------------------------------------
+//
+// Up to four positions do not fill an MFMA tile, and the latency of a stage ring is most of such a
+// call. Here a wave's lanes lie along K (16 bytes each, 512 columns a load), the four waves of a
+// workgroup take turns at the 512-column chunks, and every wave keeps R rows' loads in flight with no
+// LDS or barrier before the final sum: lanes by butterfly, waves in order. Bound by the weight stream,
+// or by launch and one trip to memory where the matrix is small. R = 8 rows of one matrix (4 of each
+// where there are two, fewer where the matrix has too few rows for the CUs).
+
+template <class T>
+__device__ __forceinline__ void widen8(const u32x4_t& v, float out[8]) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (o + q >= a.n) break;
-                    if (res != nullptr) g[q] += T::widen(res[q]);
-                    dst[q] = T::round(g[q]);
-                }
-            }
+    for (int i = 0; i < 4; ++i) {
+        out[2 * i] = T::widen(static_cast<uint16_t>(v[i] & 0xFFFFu));
+        out[2 * i + 1] = T::widen(static_cast<uint16_t>(v[i] >> 16));
+    }
+}
+
+// Dots of R weight rows with TOK rows of x over this wave's chunks of K: acc[r][t] += this lane's part.
+// Of a last chunk that K cuts, a lane loads the row's last eight values at most and masks those that
+// the lane before it has: every load stays inside its row (so K has at least eight columns).
+template <class T, int R, int TOK>
+__device__ __forceinline__ void row_dots(const uint16_t* const (&w)[R], const uint16_t* const (&x)[TOK], int k, int wave,
+                                         int waves, int lane, float (&acc)[R][TOK]) {
+    typedef u32x4_t __attribute__((aligned(2))) loose_t;
+    auto chunk = [&](int c, auto cut, u32x4_t keep) __attribute__((always_inline)) {
+        u32x4_t wv[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) wv[r] = __builtin_nontemporal_load(reinterpret_cast<const AEON_GLOBAL loose_t*>(as_global<uint16_t>(w[r]) + c));
+        float xv[TOK][8];
+#pragma unroll
+        for (int t = 0; t < TOK; ++t) {
+            u32x4_t v = *reinterpret_cast<const AEON_GLOBAL loose_t*>(as_global<uint16_t>(x[t]) + c);
+            if (cut) v &= keep;
+            widen8<T>(v, xv[t]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float wf[8];
+            if (cut) wv[r] &= keep;
+            widen8<T>(wv[r], wf);
+#pragma unroll
+            for (int t = 0; t < TOK; ++t)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) acc[r][t] = fmaf(wf[q], xv[t][q], acc[r][t]);
+        }
+    };
+    int at = wave * 512;
+    for (; at + 512 <= k; at += waves * 512) chunk(at + lane * 8, std::false_type{}, u32x4_t{});
+    if (at < k) {
+        const int c = at + lane * 8;
+        const int from = c < k - 8 ? c : k - 8;
+        u32x4_t keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            keep[i] = (from + 2 * i >= c ? 0xFFFFu : 0u) | (from + 2 * i + 1 >= c ? 0xFFFF0000u : 0u);
+        chunk(from, std::true_type{}, keep);
+    }
+}
+
+constexpr int kFewWaves = 4;
+constexpr int kFewMax = 4;  // positions of a window
+constexpr int kFewColumns = 8;
+
+template <class T, int ROWS, int MATS, int TOK>
+__device__ __forceinline__ void few_body(const ProductArgs& a, const ProductTile& t, float (*sums)[kFewWaves]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = t.row_block * ROWS;
+    const uint16_t* w[ROWS * MATS];
+#pragma unroll
+    for (int r = 0; r < ROWS * MATS; ++r) {
+        const int row = n0 + r % ROWS < a.n ? n0 + r % ROWS : a.n - 1;
+        w[r] = a.w[r / ROWS] + t.expert * a.expert_stride + row * a.w_stride;
+    }
+    const uint16_t* x[TOK];
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+        int m = t.first + (i < t.count ? i : t.count - 1);
+        if (a.rows != nullptr) {
+            m = a.rows[m];
+            m = m < 0 ? 0 : (m < a.x_rows ? m : a.x_rows - 1);
+        }
+        x[i] = a.x + m * a.x_stride;
+    }
+    float acc[ROWS * MATS][TOK] = {};
+    row_dots<T>(w, x, a.k, wave, kFewWaves, lane, acc);
+#pragma unroll
+    for (int r = 0; r < ROWS * MATS; ++r)
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+            const float v = wave_xor_sum(acc[r][i], 63);
+            if (lane == 0) sums[r * TOK + i][wave] = v;
+        }
+    __syncthreads();
+    const int i = threadIdx.x / ROWS, r = threadIdx.x % ROWS, o = n0 + r;
+    if (i >= t.count || o >= a.n) return;
+    auto total = [&](int m) {
+        const float* v = sums[(m * ROWS + r) * TOK + i];
+        float s = ((v[0] + v[1]) + v[2]) + v[3];
+        if (a.bias[m] != nullptr) s += T::widen(a.bias[m][static_cast<size_t>(t.expert) * a.n + o]);
+        return s;
+    };
+    const int p = t.first + i;
+    const float g = total(0);
+    if (a.mode == kProductDraws) {
+        const long draw = a.draws[p];
+        if (draw >= 0 && draw < a.draw_count) a.wide[static_cast<size_t>(draw) * a.n + o] = g * a.draw_weights[draw];
+        return;
+    }
+    if (a.rows != nullptr) {
+        const int row = a.rows[p];
+        if (row < 0 || row >= a.x_rows) return;
+    }
+    float y = activate(a.activation, g, MATS == 2 ? total(1) : 0.0f, a.limit);
+    if (a.residual != nullptr) y += T::widen(a.residual[p * a.residual_stride + o]);
+    a.y[p * a.y_stride + o] = T::round(y);
+}
+
+template <class T, int ROWS, int MATS>
+__global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(const ProductArgs a) {
+    __shared__ float sums[ROWS * MATS * kFewMax][kFewWaves];
+    ProductTile t;
+    if (!find_tile<kFewMax, false>(a, (a.n + ROWS - 1) / ROWS, blockIdx.x, &t)) return;
+    if (t.count == 1) few_body<T, ROWS, MATS, 1>(a, t, sums);
+    else if (t.count == 2) few_body<T, ROWS, MATS, 2>(a, t, sums);
+    else few_body<T, ROWS, MATS, 4>(a, t, sums);
+}
+
+// The weighted sum of a token's expert products in one launch: a workgroup walks the slots of its
+// token for ROWS outputs, so nothing passes through memory between the products and the sum. Every
+// slot streams its expert's rows anew, hence for a token or two. The slots' chunks of K follow each
+// other in one sequence whose next loads are issued before the present ones are used. At most 64
+// draws: lane l holds draw l's id, weight and position.
+constexpr int kDirectDraws = 64;
+constexpr int kDirectTokens = 2;
+template <class T, int ROWS>
+__global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const ProductArgs a, const int32_t* ids, int slots,
+                                                                       const uint16_t* base, long base_stride,
+                                                                       uint16_t* out, long out_stride) {
+    typedef u32x4_t __attribute__((aligned(2))) loose_t;
+    __shared__ float sums[ROWS][kFewWaves];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int token = blockIdx.y;
+    const int n0 = blockIdx.x * ROWS;
+    int listed = a.offsets[a.experts];
+    listed = listed < a.positions ? listed : a.positions;
+    const int draw_here = lane < listed ? a.draws[lane] : -1;
+    const int own = token * slots + lane;
+    const int id = lane < slots ? ids[own] : -1;
+    const float weight = lane < slots ? a.draw_weights[own] : 0.0f;
+    int position = -1;
+    for (int s = 0; s < slots; ++s) {
+        const uint64_t at = __ballot(draw_here == token * slots + s);
+        if (lane == s && at != 0) position = __builtin_ctzll(at);
+    }
+    // a slot whose id names no expert, or that no list holds, is left out
+    uint64_t slots_left = __ballot(lane < slots && id >= 0 && id < a.experts && position >= 0);
+
+    // the sequence (slot, chunk of 512 columns): this wave's chunks are wave, wave + 4, ...
+    int slot = 0, at = a.k;
+    auto next = [&]() __attribute__((always_inline)) {  // false when the sequence has ended
+        at += kFewWaves * 512;
+        if (at < a.k) return true;
+        if (wave * 512 >= a.k || slots_left == 0) return false;
+        slot = __builtin_ctzll(slots_left);
+        slots_left &= slots_left - 1;
+        at = wave * 512;
+        return true;
+    };
+    struct Load {
+        u32x4_t w[ROWS], x;
+        int slot, c;
+    } load[2];
+    auto issue = [&](Load& l) __attribute__((always_inline)) {
+        const int expert = __builtin_amdgcn_readlane(id, slot);
+        const int p = __builtin_amdgcn_readlane(position, slot);
+        const int c = at + lane * 8;
+        const int from = c < a.k - 8 ? c : a.k - 8;
+        l.slot = slot;
+        l.c = c;
+        const AEON_GLOBAL uint16_t* w = as_global<uint16_t>(a.w[0]) + expert * a.expert_stride;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int row = n0 + r < a.n ? n0 + r : a.n - 1;
+            l.w[r] = __builtin_nontemporal_load(reinterpret_cast<const AEON_GLOBAL loose_t*>(w + row * a.w_stride + from));
+        }
+        l.x = *reinterpret_cast<const AEON_GLOBAL loose_t*>(as_global<uint16_t>(a.x) + p * a.x_stride + from);
+    };
+    float total[ROWS] = {};
+    auto use = [&](Load& l) __attribute__((always_inline)) {
+        const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), l.slot));
+        u32x4_t keep;  // the values before column c are the lane before's (row_dots)
+        const int over = l.c < a.k - 8 ? 0 : l.c - (a.k - 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keep[i] = (2 * i >= over ? 0xFFFFu : 0u) | (2 * i + 1 >= over ? 0xFFFF0000u : 0u);
+        float x[8];
+        widen8<T>(l.x & keep, x);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float w[8], dot = 0.0f;
+            widen8<T>(l.w[r] & keep, w);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) dot = fmaf(w[q], x[q], dot);
+            total[r] = fmaf(scale, dot, total[r]);
+        }
+    };
+    const uint64_t all_slots = slots_left;
+    bool more = next();
+    if (more) issue(load[0]);
+    while (more) {
+        const bool second = next();
+        if (second) issue(load[1]);
+        use(load[0]);
+        if (!second) break;
+        more = next();
+        if (more) issue(load[0]);
+        use(load[1]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const float v = wave_xor_sum(total[r], 63);
+        if (lane == 0) sums[r][wave] = v;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    const int o = n0 + lane;
+    const bool live = lane < ROWS && o < a.n;
+    float y = 0.0f;
+    if (live) y = ((sums[lane][0] + sums[lane][1]) + sums[lane][2]) + sums[lane][3];
+    if (a.bias[0] != nullptr) {
+        for (uint64_t left = all_slots; left != 0; left &= left - 1) {
+            const int s = __builtin_ctzll(left);
+            const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), s));
+            const int expert = __builtin_amdgcn_readlane(id, s);
+            if (live) y = fmaf(scale, T::widen(a.bias[0][static_cast<size_t>(expert) * a.n + o]), y);
         }
     }
+    if (!live) return;
+    if (base != nullptr) y += T::widen(base[token * base_stride + o]);
+    out[token * out_stride + o] = T::round(y);
 }
 
 // Joins the shares of K of a dense product, in share order, and applies the epilogue. Four outputs
@@ -441,16 +867,17 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, 
             }
         }
     }
+    float4_t y;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        if (o + q >= a.n) break;
         float g = v[0][q], u = v[1][q];
-        if (a.bias[0] != nullptr) g += T::widen(a.bias[0][o + q]);
-        if (a.pair && a.bias[1] != nullptr) u += T::widen(a.bias[1][o + q]);
-        g = activate(a.activation, g, u, a.limit);
-        if (a.residual != nullptr) g += T::widen(a.residual[p * a.residual_stride + o + q]);
-        a.y[p * a.y_stride + o + q] = T::round(g);
+        if (o + q < a.n) {
+            if (a.bias[0] != nullptr) g += T::widen(a.bias[0][o + q]);
+            if (a.bias[1] != nullptr) u += T::widen(a.bias[1][o + q]);
+        }
+        y[q] = activate(a.activation, g, u, a.limit);
     }
+    finish<T>(a, p, o, y);
 }
 
 // out[t][i] = round(base[t][i] + sum of the token's contributions in slot order). A draw whose id
@@ -514,11 +941,33 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
     // an upper bound of the windows: every list that holds something may end in a short one
     long windows = (static_cast<long>(a.positions) + BM - 1) / BM;
     if (a.offsets != nullptr) windows = a.positions / BM + (a.experts < a.positions ? a.experts : a.positions);
-    const long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
+    long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
+    if (BM == 256 && ALIGNED) grid += kXcds * (kXcdCus / 2);  // room for a last round in halves
     AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
     kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(a);
     AEON_LAUNCH_CHECK();
     return AEON_OK;
+}
+
+// Rows of each matrix a workgroup of the few-position kernel takes: eight loads in flight a wave, or
+// fewer where that would leave CUs without a workgroup.
+template <class T, int ROWS, int MATS>
+static int launch_few_rows(const ProductArgs& a, long windows, hipStream_t stream) {
+    const long grid = (windows * ((a.n + ROWS - 1) / ROWS) + kXcds - 1) / kXcds * kXcds;
+    AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
+    product_few_kernel<T, ROWS, MATS><<<static_cast<unsigned>(grid), 64 * kFewWaves, 0, stream>>>(a);
+    AEON_LAUNCH_CHECK();
+    return AEON_OK;
+}
+
+template <class T>
+static int launch_few(const ProductArgs& a, hipStream_t stream) {
+    long windows = (static_cast<long>(a.positions) + kFewMax - 1) / kFewMax;
+    if (a.offsets != nullptr) windows = a.positions / kFewMax + (a.experts < a.positions ? a.experts : a.positions);
+    const long rows = windows * a.n;
+    if (a.pair) return rows >= 4 * 512 ? launch_few_rows<T, 4, 2>(a, windows, stream) : launch_few_rows<T, 1, 2>(a, windows, stream);
+    if (rows >= 8 * 512) return launch_few_rows<T, 8, 1>(a, windows, stream);
+    return rows >= 4 * 512 ? launch_few_rows<T, 4, 1>(a, windows, stream) : launch_few_rows<T, 1, 1>(a, windows, stream);
 }
 
 template <class T, bool ALIGNED>
@@ -548,6 +997,7 @@ static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipSt
                          a.x_stride % 8 == 0 && a.w_stride % 8 == 0 && a.expert_stride % 8 == 0;
     a.vec_out = a.n % 4 == 0 && a.y_stride % 4 == 0 && on_boundary(a.y, 8) && a.residual_stride % 4 == 0 &&
                 on_boundary(a.residual, 8);
+    if (tile == kFewMax) return dtype == AEON_DTYPE_F16 ? launch_few<F16>(a, stream) : launch_few<BF16>(a, stream);
     if (dtype == AEON_DTYPE_F16) {
         return aligned ? launch_tiles<F16, true>(tile, a, splits, stream) : launch_tiles<F16, false>(tile, a, splits, stream);
     }
@@ -564,6 +1014,7 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
     const long n = static_cast<long>(w.out_dim) * (pair ? 2 : 1);
     auto tiles = [&](long bm, long bn) { return (tokens + bm - 1) / bm * ((n + bn - 1) / bn); };
     ProductPlan p{16, 1, 0};
+    if (tokens <= kFewMax && w.in_dim >= kFewColumns) return ProductPlan{kFewMax, 1, 0};
     if (tokens > 16) p.tile = 32;
     if (tokens > 32) p.tile = 64;
     if (tokens > 64 && tiles(128, 128) >= 256) p.tile = 128;
@@ -581,7 +1032,8 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
 }
 
 // Experts: by how many positions an expert holds on average.
-static int plan_experts(int positions, int experts) {
+static int plan_experts(const aeon_projection& w, int positions, int experts) {
+    if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kFewMax;
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
     return mean <= 8 ? 16 : mean <= 24 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
@@ -632,6 +1084,10 @@ static int check_experts(const aeon_projection& w, int experts, long expert_stri
     AEON_REQUIRE(expert_stride >= (w.out_dim - 1) * w.weight_stride + w.in_dim, AEON_ERR_INVALID_ARGUMENT,
                  "%s: expert matrices %ld elements apart overlap", who, expert_stride);
     return AEON_OK;
+}
+
+static bool combine_direct(const aeon_projection& w, int tokens, int slots) {
+    return tokens <= kDirectTokens && static_cast<long>(tokens) * slots <= kDirectDraws && w.in_dim >= kFewColumns;
 }
 
 static size_t linear_workspace(const aeon_projection& w, int tokens, const ProductPlan& p) {
@@ -722,11 +1178,12 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
     a.positions = positions;
     a.y = static_cast<uint16_t*>(d_y);
     a.y_stride = y_stride;
-    return launch_product(w.dtype, plan_experts(positions, experts), a, 1, as_stream(stream));
+    return launch_product(w.dtype, plan_experts(w, positions, experts), a, 1, as_stream(stream));
 }
 
 extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots) {
     if (check_projection(projection, "aeon_expert_combine_workspace_bytes") != AEON_OK || tokens <= 0 || slots <= 0) return 0;
+    if (combine_direct(*projection, tokens, slots)) return 0;
     return static_cast<size_t>(tokens) * slots * projection->out_dim * sizeof(float);
 }
 
@@ -756,8 +1213,8 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
     AEON_REQUIRE(d_out != d_base || out_stride == base_stride, AEON_ERR_INVALID_ARGUMENT,
                  "%s: an output on the base needs the base's row pitch", who);
     const size_t need = aeon_expert_combine_workspace_bytes(projection, tokens, slots);
-    AEON_REQUIRE(workspace_bytes >= need && d_workspace != nullptr && on_boundary(d_workspace, 16), AEON_ERR_INVALID_ARGUMENT,
-                 "%s: needs a workspace of %zu bytes on a 16-byte boundary (%zu given)", who, need, workspace_bytes);
+    AEON_REQUIRE(workspace_bytes >= need && (need == 0 || (d_workspace != nullptr && on_boundary(d_workspace, 16))),
+                 AEON_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes on a 16-byte boundary (%zu given)", who, need, workspace_bytes);
     ProductArgs a = projection_args(w);
     a.expert_stride = expert_stride;
     a.x = static_cast<const uint16_t*>(d_h);
@@ -771,12 +1228,21 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
     a.draws = d_draw_indices;
     a.draw_weights = d_topk_weights;
     a.draw_count = tokens * slots;
-    if (int rc = launch_product(w.dtype, plan_experts(a.positions, experts), a, 1, as_stream(stream))) return rc;
+    const auto* base = static_cast<const uint16_t*>(d_base);
+    auto* out = static_cast<uint16_t*>(d_out);
+    if (combine_direct(w, tokens, slots)) {
+        const dim3 grid((w.out_dim + 7) / 8, tokens);
+        if (w.dtype == AEON_DTYPE_F16)
+            product_token_kernel<F16, 8><<<grid, 64 * kFewWaves, 0, as_stream(stream)>>>(a, d_topk_ids, slots, base, base_stride, out, out_stride);
+        else
+            product_token_kernel<BF16, 8><<<grid, 64 * kFewWaves, 0, as_stream(stream)>>>(a, d_topk_ids, slots, base, base_stride, out, out_stride);
+        AEON_LAUNCH_CHECK();
+        return AEON_OK;
+    }
+    if (int rc = launch_product(w.dtype, plan_experts(w, a.positions, experts), a, 1, as_stream(stream))) return rc;
     const long threads = static_cast<long>(tokens) * ((w.out_dim + 3) / 4);
     AEON_REQUIRE((threads + 255) / 256 <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "%s: too many outputs for one launch", who);
     const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-    const auto* base = static_cast<const uint16_t*>(d_base);
-    auto* out = static_cast<uint16_t*>(d_out);
     if (w.dtype == AEON_DTYPE_F16) {
         product_combine_kernel<F16><<<blocks, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, tokens, slots, w.out_dim,
                                                                           base, base_stride, out, out_stride);

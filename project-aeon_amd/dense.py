@@ -29,23 +29,27 @@ class Projection(C.Structure):
                 ("d_bias", C.c_void_p), ("d_bias_up", C.c_void_p), ("swiglu_limit", C.c_float)]
 
 
-def _check(t, name, like, shape, dtype=None):
-    """One operand: on x's GPU, of its type (or `dtype`), of this shape, its rows contiguous."""
-    dtype = like.dtype if dtype is None else dtype
-    if t.dtype != dtype:
+# These functions are called once per projection and token: what they check, they check with a few attribute
+# reads, and one call costs the host about as much as one of torch's own element-wise operators.
+
+
+def _check(t, name, device, dtype, shape):
+    """One operand: of this type, on this GPU, of this shape, the elements of a row next to each other."""
+    if t.dtype is not dtype:
         raise ValueError("%s is %s, not %s" % (name, t.dtype, dtype))
-    if t.device != like.device:
-        raise ValueError("%s is on %s, not on %s" % (name, t.device, like.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.get_device() != device:
+        raise ValueError("%s is on %s, not on GPU %d" % (name, t.device, device))
+    if t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError("%s: elements of a row have to follow each other" % name)
-    return t
 
 
 def _pitch(t):
     """Row pitch of a 2-d tensor: a tensor of one row may carry any stride for it."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, cols = t.shape
+    pitch = t.stride(0)
+    return pitch if rows > 1 or pitch > cols else cols
 
 
 def _ptr(t):
@@ -53,45 +57,53 @@ def _ptr(t):
 
 
 def _projection(x, weight, bias, activation, weight_up, bias_up, limit, lead):
-    if x.dim() != 2 or x.dtype not in _DTYPES or not x.is_cuda:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or x.dim() != 2 or not x.is_cuda:
         raise ValueError("x has to be a 2-d fp16 or bf16 tensor on a GPU")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError("unknown activation %r" % (activation,))
-    if weight.dim() != 2 + lead:
+    shape = weight.shape
+    if len(shape) != 2 + lead:
         raise ValueError("weight has to have %d dimensions" % (2 + lead))
-    out_dim, in_dim = weight.shape[-2:]
-    _check(x, "x", x, (x.shape[0], in_dim))
-    _check(weight, "weight", x, weight.shape)
-    stride = weight.stride(-2) if out_dim > 1 else max(weight.stride(-2), in_dim)
+    out_dim, in_dim = shape[-2], shape[-1]
+    device = x.get_device()
+    _check(x, "x", device, x.dtype, (x.shape[0], in_dim))
+    _check(weight, "weight", device, x.dtype, shape)
+    stride = weight.stride(-2)
+    if out_dim == 1 and stride < in_dim:
+        stride = in_dim
     if weight_up is not None:
-        _check(weight_up, "weight_up", x, weight.shape)
+        _check(weight_up, "weight_up", device, x.dtype, shape)
         if weight_up.stride() != weight.stride():
             raise ValueError("weight and weight_up have to have the same strides")
     for b, name in ((bias, "bias"), (bias_up, "bias_up")):
         if b is not None:
-            _check(b, name, x, weight.shape[:-1])
+            _check(b, name, device, x.dtype, shape[:-1])
             if not b.is_contiguous():
                 raise ValueError("%s has to be contiguous" % name)
-    return Projection(_DTYPES[x.dtype], in_dim, out_dim, ACTIVATIONS[activation], weight.data_ptr(), _ptr(weight_up),
-                      stride, _ptr(bias), _ptr(bias_up), limit)
+    return Projection(dtype, in_dim, out_dim, act, weight.data_ptr(), _ptr(weight_up), stride, _ptr(bias), _ptr(bias_up), limit)
 
 
-def _call(x, name, *args):
-    """One entry point on the current stream of x's GPU, with that GPU current."""
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    if x.device.index == torch.cuda.current_device():
-        capi.call(name, *args, C.c_void_p(stream))
+def _call(device, name, *args):
+    """One entry point on the current stream of a GPU, with that GPU current."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch.cuda.current_device():
+        capi.call(name, *args, stream)
     else:
-        with torch.cuda.device(x.device):
-            capi.call(name, *args, C.c_void_p(stream))
+        with torch.cuda.device(device):
+            capi.call(name, *args, stream)
 
 
 def _output(out, x, shape):
-    return torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else _check(out, "out", x, shape)
+    if out is None:
+        return x.new_empty(shape)
+    _check(out, "out", x.get_device(), x.dtype, shape)
+    return out
 
 
 def _workspace(x, need):
-    return torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    return x.new_empty(need, dtype=torch.uint8) if need else None
 
 
 def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None, swiglu_limit=float("inf"),
@@ -99,15 +111,16 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
     """act(x @ weight.T + bias) + residual (aeon_linear). x [tokens][in_dim], weight [out_dim][in_dim];
     "swiglu" takes the second matrix as weight_up. `out` may be the residual itself."""
     p = _projection(x, weight, bias, activation, weight_up, bias_up, swiglu_limit, 0)
-    shape = (x.shape[0], p.out_dim)
+    device, tokens = x.get_device(), x.shape[0]
+    shape = (tokens, p.out_dim)
     if residual is not None:
-        _check(residual, "residual", x, shape)
+        _check(residual, "residual", device, x.dtype, shape)
     out = _output(out, x, shape)
-    need = capi.lib().aeon_linear_workspace_bytes(C.byref(p), shape[0])
+    at = C.addressof(p)
+    need = capi.lib().aeon_linear_workspace_bytes(at, tokens)
     ws = _workspace(x, need)
-    _call(x, "aeon_linear", C.byref(p), capi.vp(x), C.c_long(_pitch(x)), shape[0], capi.vp(residual),
-          C.c_long(0 if residual is None else _pitch(residual)), capi.vp(out), C.c_long(_pitch(out)), capi.vp(ws),
-          C.c_size_t(need))
+    _call(device, "aeon_linear", at, x.data_ptr(), _pitch(x), tokens, _ptr(residual),
+          0 if residual is None else _pitch(residual), out.data_ptr(), _pitch(out), _ptr(ws), need)
     return out
 
 
@@ -119,20 +132,22 @@ def expert_lists(ids, experts):
         raise ValueError("ids has to be a contiguous int32 tensor [tokens][slots] on a GPU")
     new = lambda n: torch.empty(n, dtype=torch.int32, device=ids.device)
     lists = ExpertLists(new(experts + 1), new(ids.numel()), new(ids.numel()))
-    _call(ids, "aeon_expert_permutation", capi.vp(ids), ids.shape[0], ids.shape[1], experts, capi.vp(lists.offsets),
-          capi.vp(lists.rows), capi.vp(lists.draws), None, None)
+    stream = lambda: C.c_void_p(torch.cuda.current_stream(ids.device).cuda_stream)
+    with torch.cuda.device(ids.device):
+        capi.call("aeon_expert_permutation", capi.vp(ids), ids.shape[0], ids.shape[1], experts, capi.vp(lists.offsets),
+                  capi.vp(lists.rows), capi.vp(lists.draws), None, None, stream())
     return lists
 
 
-def _lists(x, experts, offsets, positions, **more):
-    _check(offsets, "offsets", x, (experts + 1,), torch.int32)
-    for name, t in more.items():
-        if t is not None:
-            _check(t, name, x, (positions,), torch.int32)
+def _lists(device, experts, offsets, positions, lists, name):
+    _check(offsets, "offsets", device, torch.int32, (experts + 1,))
+    if lists is not None:
+        _check(lists, name, device, torch.int32, (positions,))
 
 
 def _expert_stride(weight, p):
-    return weight.stride(0) if weight.shape[0] > 1 else max(weight.stride(0), p.out_dim * p.weight_stride)
+    stride = weight.stride(0)
+    return stride if weight.shape[0] > 1 else max(stride, p.out_dim * p.weight_stride)
 
 
 def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", weight_up=None, bias_up=None,
@@ -141,12 +156,12 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
     positions are offsets[e] .. offsets[e+1]-1, position p takes row rows[p] of x (without `rows`: row p).
     Returns [positions][out_dim]; rows behind the last list are not written."""
     p = _projection(x, weight, bias, activation, weight_up, bias_up, swiglu_limit, 1)
-    positions = x.shape[0] if rows is None else rows.shape[0]
-    _lists(x, weight.shape[0], offsets, positions, rows=rows)
+    device, x_rows = x.get_device(), x.shape[0]
+    positions = x_rows if rows is None else rows.shape[0]
+    _lists(device, weight.shape[0], offsets, positions, rows, "rows")
     out = _output(out, x, (positions, p.out_dim))
-    _call(x, "aeon_expert_linear", C.byref(p), weight.shape[0], C.c_long(_expert_stride(weight, p)), capi.vp(x),
-          C.c_long(_pitch(x)), x.shape[0], capi.vp(offsets), capi.vp(rows), positions, capi.vp(out),
-          C.c_long(_pitch(out)))
+    _call(device, "aeon_expert_linear", C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), _pitch(x),
+          x_rows, offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), _pitch(out))
     return out
 
 
@@ -158,19 +173,22 @@ def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None
     if ids.dim() != 2:
         raise ValueError("ids has to be [tokens][slots]")
     tokens, slots = ids.shape
-    _check(h, "h", h, (tokens * slots, p.in_dim))
-    _lists(h, weight.shape[0], offsets, tokens * slots, draws=draws)
-    _check(ids, "ids", h, (tokens, slots), torch.int32)
-    _check(weights, "weights", h, (tokens, slots), torch.float32)
+    device = h.get_device()
+    if h.shape[0] != tokens * slots:
+        raise ValueError("h has %d rows, not %d" % (h.shape[0], tokens * slots))
+    _lists(device, weight.shape[0], offsets, tokens * slots, draws, "draws")
+    _check(ids, "ids", device, torch.int32, ids.shape)
+    _check(weights, "weights", device, torch.float32, ids.shape)
     if not (ids.is_contiguous() and weights.is_contiguous()):
         raise ValueError("ids and weights have to be contiguous")
+    shape = (tokens, p.out_dim)
     if base is not None:
-        _check(base, "base", h, (tokens, p.out_dim))
-    out = _output(out, h, (tokens, p.out_dim))
-    need = capi.lib().aeon_expert_combine_workspace_bytes(C.byref(p), tokens, slots)
+        _check(base, "base", device, h.dtype, shape)
+    out = _output(out, h, shape)
+    at = C.addressof(p)
+    need = capi.lib().aeon_expert_combine_workspace_bytes(at, tokens, slots)
     ws = _workspace(h, need)
-    _call(h, "aeon_expert_combine", C.byref(p), weight.shape[0], C.c_long(_expert_stride(weight, p)), capi.vp(h),
-          C.c_long(_pitch(h)), capi.vp(offsets), capi.vp(draws), capi.vp(ids), capi.vp(weights), tokens, slots,
-          capi.vp(base), C.c_long(0 if base is None else _pitch(base)), capi.vp(out), C.c_long(_pitch(out)),
-          capi.vp(ws), C.c_size_t(need))
+    _call(device, "aeon_expert_combine", at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), _pitch(h),
+          offsets.data_ptr(), draws.data_ptr(), ids.data_ptr(), weights.data_ptr(), tokens, slots, _ptr(base),
+          0 if base is None else _pitch(base), out.data_ptr(), _pitch(out), _ptr(ws), need)
     return out

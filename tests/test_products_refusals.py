@@ -62,11 +62,11 @@ def test_linear_refusals(kw, text):
 
 def test_linear_refuses_a_short_workspace():
     p = _p(in_dim=7168, weight_stride=7168, out_dim=256)
-    need = capi.lib().aeon_linear_workspace_bytes(C.byref(p), 1)
+    need = capi.lib().aeon_linear_workspace_bytes(C.byref(p), 20)
     assert need > 0 and need % (256 * 4) == 0
     for ws, wb in ((None, need), (A, need - 1), (C.c_void_p((1 << 20) + 4), need)):
         with pytest.raises(ValueError, match="workspace of"):
-            _linear(p, xs=7168, ys=256, tokens=1, ws=ws, wb=wb)
+            _linear(p, xs=7168, ys=256, tokens=20, ws=ws, wb=wb)
 
 
 @pytest.mark.parametrize("kw,text", [
