@@ -453,21 +453,24 @@ int aeon_linear(const aeon_projection* projection, const void* d_x, long x_strid
  * expert_offsets[e+1]-1 are its list (aeon_expert_permutation), so that
  * y[p] = round(act(W_e x[row_indices[p]] + bias_e)); without row_indices row p itself. d_x has x_rows
  * rows. Rows of y behind the last list, and those of a position whose row index is outside
- * [0, x_rows), are left as they were. An expert without positions is not read. */
+ * [0, x_rows), are left as they were. An expert without positions is not read. The workspace (16-byte
+ * boundary) holds the tiles of long lists; short ones need none. */
+size_t aeon_expert_linear_workspace_bytes(const aeon_projection* projection, int experts, int positions);
 int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,
                        const void* d_x, long x_stride, int x_rows, const int32_t* d_expert_offsets,
                        const int32_t* d_row_indices, int positions, void* d_y, long y_stride,
-                       void* stream);
+                       void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* The down projection and the way back to tokens, the unquantised counterpart of
  * dispatch_aeon_moe_grouped_w2_wmma + the fixed-order reduce (moe_grouped_dispatch.hpp:66-88,
  * src/architecture/deepseek_v4/moe/moe_grouped_batch.hpp:119-146):
  * out[t] = round(base[t] + sum over s ascending of weights[t][s] * (W_e h[p] + bias_e)), where p is the
  * position whose draw_indices[p] is t*slots + s, and e = ids[t][s] the expert that lists it. The
- * contributions stay fp32 (workspace, tokens * slots * out_dim floats). A slot whose id is outside
+ * contributions stay fp32 (in the workspace, 16-byte boundary; a token or two need none). A slot whose id is outside
  * [0, experts) contributes nothing. d_base is nullable and may be d_out (same pitch). The projection
  * has no activation. d_h has tokens * slots rows, by position. */
-size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots);
+size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int experts, int tokens,
+                                           int slots);
 int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,
                         const void* d_h, long h_stride, const int32_t* d_expert_offsets,
                         const int32_t* d_draw_indices, const int32_t* d_topk_ids,

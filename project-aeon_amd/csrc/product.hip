@@ -24,6 +24,7 @@
 namespace aeon355 {
 
 typedef __bf16 bf16_t;
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 template <int N>
@@ -42,6 +43,9 @@ struct F16 {
     }
     static __device__ __forceinline__ float widen(uint16_t v) { return half_bits_to_float(v); }
     static __device__ __forceinline__ uint16_t round(float v) { return float_to_half_bits(v); }
+    static __device__ __forceinline__ uint32_t round2(float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(lo), static_cast<half_t>(hi)});
+    }
 };
 struct BF16 {
     static __device__ __forceinline__ float4_t mfma(const u32x4_t& a, const u32x4_t& b, const float4_t& c) {
@@ -54,24 +58,46 @@ struct BF16 {
     static __device__ __forceinline__ uint16_t round(float v) {  // to nearest even, NaN kept
         return __builtin_bit_cast(uint16_t, static_cast<bf16_t>(v));
     }
+    static __device__ __forceinline__ uint32_t round2(float lo, float hi) {
+        return __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<bf16_t>(lo), static_cast<bf16_t>(hi)});
+    }
 };
 
-// Activations in fp32. The clamps are comparisons, not fminf/fmaxf: those return the bound for a
-// NaN operand and would turn a NaN pre-activation into a finite value.
-__device__ __forceinline__ float activate(int kind, float g, float u, float limit) {
+// 1 / (1 + exp(-z)): the exponential by the hardware's power of two. z * log2(e) is rounded to 24
+// bits, which shifts the exponential by at most |z| * 2^-24 of itself; the result is rounded to 11 bits
+// or fewer. Saturates to 0 and 1 without NaN.
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+
+// Activations in fp32, in place on N values. gelu_tanh is g * sigmoid(2z), as (1 + tanh z) / 2 is
+// sigmoid(2z), without the cancellation. The clamps are comparisons, not fminf/fmaxf: those return
+// the bound for a NaN operand and would turn a NaN pre-activation into a finite value.
+template <int N>
+__device__ __forceinline__ void activate(int kind, float (&g)[N], const float (&u)[N], float limit) {
     switch (kind) {
-        case AEON_ACT_SILU: return g / (1.0f + expf(-g));
-        case AEON_ACT_GELU: return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-        case AEON_ACT_GELU_TANH: {
-            const float z = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-            return 0.5f * g * (1.0f + tanhf(z));
-        }
-        case AEON_ACT_SWIGLU: {
-            g = g > limit ? limit : g;
-            u = u > limit ? limit : (u < -limit ? -limit : u);
-            return g / (1.0f + expf(-g)) * u;
-        }
-        default: return g;
+        case AEON_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] *= sigmoid(g[i]);
+            break;
+        case AEON_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] *= 0.5f * (1.0f + erff(g[i] * 0.70710678118654752f));
+            break;
+        case AEON_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                g[i] *= sigmoid(2.0f * 0.79788456080286536f * (g[i] + 0.044715f * g[i] * g[i] * g[i]));
+            break;
+        case AEON_ACT_SWIGLU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = g[i] > limit ? limit : g[i];
+                const float y = u[i] > limit ? limit : (u[i] < -limit ? -limit : u[i]);
+                g[i] = x * sigmoid(x) * y;
+            }
+            break;
+        default: break;
     }
 }
 
@@ -106,40 +132,54 @@ struct ProductTile {
     bool only;                            // no other window of the list reads these rows
 };
 
-// Tile of workgroup b. Workgroups are dealt to the 8 XCDs round robin, so tile numbers are handed
-// out in 8 contiguous runs, one per XCD: neighbouring tiles share panels through one L2. Inside an
-// expert up to kWindowGroup windows take turns over each row block, a near-square patch of the
-// output for the workgroups that run at the same time.
-// HALVES: one workgroup fills a CU, and a tile may be run as two of half the positions at half the
-// cost each. Where at most half of the CUs would have a tile in an XCD's last round, the tiles of that
-// round are cut so.
-template <int BM, bool HALVES>
-__device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, int b, ProductTile* t) {
-    const int lane = threadIdx.x & 63;
-    int expert = 0, first = 0, held = a.positions, before = 0, windows;
-    int total;
-    if (a.offsets == nullptr) {
-        windows = (held + BM - 1) / BM;
-        total = windows * row_blocks;
-    }
-    const int per = a.offsets == nullptr ? 0 : (a.experts + 63) / 64;
-    int mine = 0, upto = 0;
-    // list bounds as the caller gave them, held inside [0, positions] and ascending
-    auto bound = [&](int e) {
-        const int v = a.offsets[e];
+// List of expert e as the caller gave it, held inside [0, positions].
+__device__ __forceinline__ int list_of(const ProductArgs& a, int e, int* first) {
+    auto bound = [&](int i) {
+        const int v = a.offsets[i];
         return v < 0 ? 0 : (v > a.positions ? a.positions : v);
     };
-    auto windows_of = [&](int e, int* lo, int* n) {
-        *lo = bound(e);
-        *n = bound(e + 1) - *lo;
-        if (*n < 0) *n = 0;
-        return (*n + BM - 1) / BM;
-    };
-    if (a.offsets != nullptr) {
-        for (int i = 0; i < per; ++i) {
-            const int e = lane * per + i;
-            int lo, n;
-            if (e < a.experts) mine += windows_of(e, &lo, &n);
+    *first = bound(e);
+    const int n = bound(e + 1) - *first;
+    return n > 0 ? n : 0;
+}
+
+// Window and row block of a list's tile u: up to kWindowGroup windows take turns over each row
+// block, a near-square patch of the output for the workgroups that run at the same time.
+__device__ __forceinline__ void patch_of(int u, int windows, int row_blocks, int* window, int* row_block) {
+    const int group = u / (kWindowGroup * row_blocks);
+    const int v = u - group * kWindowGroup * row_blocks;
+    const int left = windows - group * kWindowGroup;
+    const int wide = left < kWindowGroup ? left : kWindowGroup;
+    *window = group * kWindowGroup + v % wide;
+    *row_block = v / wide;
+}
+
+// Tile of workgroup b. Workgroups are dealt to the 8 XCDs round robin, so tiles are handed out in 8
+// contiguous runs, one per XCD: neighbouring tiles share panels through one L2.
+// TURNS: one workgroup fills a CU, and a tile with at most half of its positions costs half. Where at
+// most half of the CUs would have a tile in an XCD's last round, a dense product's tiles of that round
+// are cut in two (the second part of a short one is empty); the tiles of lists come from a table.
+template <int BM, bool TURNS>
+__device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, int b, ProductTile* t) {
+    if (TURNS && a.tiles != nullptr) {
+        const int4 entry = a.tiles[b];
+        t->expert = entry.x;
+        t->first = entry.y;
+        t->count = entry.z;
+        t->row_block = entry.w;
+        t->only = false;
+        return entry.z > 0;
+    }
+    const int lane = threadIdx.x & 63;
+    const bool lists = !TURNS && a.offsets != nullptr;
+    const int per = lists ? (a.experts + 63) / 64 : 0;  // experts a lane looks after
+    int mine = 0, upto = 0, total;
+    if (!lists) {
+        total = (a.positions + BM - 1) / BM * row_blocks;
+    } else {
+        for (int e = lane * per; e < (lane + 1) * per && e < a.experts; ++e) {
+            int first;
+            mine += (list_of(a, e, &first) + BM - 1) / BM;
         }
         upto = mine;
 #pragma unroll
@@ -151,7 +191,7 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
     }
     const int run = (total + kXcds - 1) / kXcds;
     int at = b / kXcds, half = -1;
-    if (HALVES) {
+    if (TURNS) {
         const int last = run % kXcdCus;
         if (last <= kXcdCus / 2 && at >= run - last) {
             half = (at - (run - last)) & 1;
@@ -160,19 +200,14 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
     }
     const int tile = (b % kXcds) * run + at;
     if (at >= run || tile >= total) return false;
-    if (a.offsets != nullptr) {
-        const int lo_tile = (upto - mine) * row_blocks;
-        const uint64_t owner = __ballot(tile >= lo_tile && tile < upto * row_blocks);
-        const int from = __builtin_ctzll(owner);
+    int expert = 0, first = 0, held = a.positions, before = 0;
+    if (lists) {
         before = upto - mine;
-        for (int i = 0; i < per; ++i) {
-            const int e = lane * per + i;
-            if (e >= a.experts) break;
-            int lo, n;
-            const int w = windows_of(e, &lo, &n);
+        const int from = __builtin_ctzll(__ballot(tile >= before * row_blocks && tile < upto * row_blocks));
+        for (int e = lane * per; e < (lane + 1) * per && e < a.experts; ++e) {
             expert = e;
-            first = lo;
-            held = n;
+            held = list_of(a, e, &first);
+            const int w = (held + BM - 1) / BM;
             if (tile < (before + w) * row_blocks) break;
             before += w;
         }
@@ -180,26 +215,95 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
         first = __builtin_amdgcn_readlane(first, from);
         held = __builtin_amdgcn_readlane(held, from);
         before = __builtin_amdgcn_readlane(before, from);
-        windows = (held + BM - 1) / BM;
     }
-    const int u = tile - before * row_blocks;
-    const int group = u / (kWindowGroup * row_blocks);
-    const int v = u - group * kWindowGroup * row_blocks;
-    const int left = windows - group * kWindowGroup;
-    const int wide = left < kWindowGroup ? left : kWindowGroup;
-    const int window = group * kWindowGroup + v % wide;
+    const int windows = (held + BM - 1) / BM;
+    int window;
+    patch_of(tile - before * row_blocks, windows, row_blocks, &window, &t->row_block);
     t->expert = expert;
-    t->row_block = v / wide;
     t->only = windows == 1;
     t->first = first + window * BM;
-    const int rest = held - window * BM;
-    t->count = rest < BM ? rest : BM;
-    if (HALVES && half >= 0) {
+    t->count = held - window * BM < BM ? held - window * BM : BM;
+    if (half >= 0) {
         t->first += half * (BM / 2);
         t->count -= half * (BM / 2);
         if (half == 0 && t->count > BM / 2) t->count = BM / 2;
     }
     return t->count > 0;
+}
+
+// The tiles of lists for the kernel whose workgroups fill a CU, one entry a workgroup: {expert, first
+// position, positions (0: nothing to do), row block}. A list is its windows of more than half the
+// positions, then perhaps one shorter that costs half. The XCDs' runs are cut at equal cost: with the
+// popular experts first, equal numbers of tiles gave the first XCD a fifth more work than the mean.
+// One workgroup, a thread an expert, then the threads over the entries.
+__global__ __launch_bounds__(1024) void product_tiles_kernel(const ProductArgs a, int bm, int row_blocks, int entries,
+                                                             int4* table) {
+    __shared__ int cost_before[1025], tiles_before[1025], wave_cost[16], wave_tiles[16], run_from[kXcds + 1];
+    const int e = threadIdx.x, lane = e & 63, wave = e >> 6;
+    auto wholes_of = [&](int n) { return n / bm + (n % bm > bm / 2); };
+    auto windows_of = [&](int n) { return (n + bm - 1) / bm; };
+    int first, held = 0;
+    if (e < a.experts) held = list_of(a, e, &first);
+    int cost = wholes_of(held) + windows_of(held), tiles = windows_of(held);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int c = __shfl_up(cost, d, 64), n = __shfl_up(tiles, d, 64);
+        if (lane >= d) {
+            cost += c;
+            tiles += n;
+        }
+    }
+    if (lane == 63) {
+        wave_cost[wave] = cost;
+        wave_tiles[wave] = tiles;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        cost += wave_cost[w];
+        tiles += wave_tiles[w];
+    }
+    cost_before[e + 1] = cost;
+    tiles_before[e + 1] = tiles;
+    if (e == 0) cost_before[0] = tiles_before[0] = 0;
+    __syncthreads();
+    auto holder = [&](const int* before, int v) {  // the expert whose share of the prefix holds v
+        int lo = 0, hi = 1024;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid] * row_blocks <= v) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    if (e <= kXcds) {  // the first tile that starts at an eighth of the cost or later
+        const int all = cost_before[1024] * row_blocks;
+        const int c = static_cast<int>(static_cast<long>(all) * e / kXcds);
+        int tile = tiles_before[1024] * row_blocks;
+        if (c < all) {
+            const int x = holder(cost_before, c);
+            int dummy;
+            const int in = c - cost_before[x] * row_blocks;
+            const int whole_cost = 2 * wholes_of(list_of(a, x, &dummy)) * row_blocks;
+            tile = tiles_before[x] * row_blocks + (in <= whole_cost ? (in + 1) / 2 : whole_cost / 2 + in - whole_cost);
+        }
+        run_from[e] = tile;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < entries; b += 1024) {
+        const int tile = run_from[b % kXcds] + b / kXcds;
+        int4 entry = make_int4(0, 0, 0, 0);
+        if (tile < run_from[b % kXcds + 1]) {
+            const int x = holder(tiles_before, tile);
+            int from;
+            const int n = list_of(a, x, &from), wholes = wholes_of(n);
+            const int u = tile - tiles_before[x] * row_blocks;
+            int window = wholes, block = u - wholes * row_blocks;
+            if (block < 0) patch_of(u, wholes, row_blocks, &window, &block);
+            const int rest = n - window * bm;
+            entry = make_int4(x, from + window * bm, rest < bm ? rest : bm, block);
+        }
+        table[b] = entry;
+    }
 }
 
 // 16 bytes of a row starting at column c, zeros from column k on. `p` is the row's column 0; nothing
@@ -230,32 +334,34 @@ __device__ __forceinline__ void store_wide(float* dst, const float4_t& v, int o,
     }
 }
 
-// The residual and the one rounding, outputs o .. o + 3 of position p.
+// Four values of one 16-bit type from p on, zeros past the row's end.
 template <class T>
-__device__ __forceinline__ void finish(const ProductArgs& a, int p, int o, float4_t g) {
-    uint16_t* dst = a.y + p * a.y_stride + o;
-    const uint16_t* res = a.residual == nullptr ? nullptr : a.residual + p * a.residual_stride + o;
-    if (a.vec_out) {
-        if (res != nullptr) {
-            const uint2 r = *reinterpret_cast<const uint2*>(res);
-            g[0] += T::widen(r.x & 0xFFFFu);
-            g[1] += T::widen(r.x >> 16);
-            g[2] += T::widen(r.y & 0xFFFFu);
-            g[3] += T::widen(r.y >> 16);
-        }
-        uint2 v;
-        v.x = T::round(g[0]) | (static_cast<uint32_t>(T::round(g[1])) << 16);
-        v.y = T::round(g[2]) | (static_cast<uint32_t>(T::round(g[3])) << 16);
-        *reinterpret_cast<uint2*>(dst) = v;
+__device__ __forceinline__ float4_t load_narrow(const uint16_t* p, bool vec, int o, int n) {
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (vec) {
+        const uint2 r = *reinterpret_cast<const uint2*>(p);
+        v = float4_t{T::widen(r.x & 0xFFFFu), T::widen(r.x >> 16), T::widen(r.y & 0xFFFFu), T::widen(r.y >> 16)};
     } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (o + q >= a.n) break;
-            if (res != nullptr) g[q] += T::widen(res[q]);
-            dst[q] = T::round(g[q]);
-        }
+        for (int q = 0; q < 4; ++q)
+            if (o + q < n) v[q] = T::widen(p[q]);
+    }
+    return v;
+}
+// The one rounding.
+template <class T>
+__device__ __forceinline__ void store_narrow(uint16_t* p, const float4_t& v, bool vec, int o, int n) {
+    if (vec) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(T::round2(v[0], v[1]), T::round2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (o + q < n) p[q] = T::round(v[q]);
     }
 }
+
+// The tile that fills a CU is run by waves that take turns (below).
+constexpr bool takes_turns(int bm, bool aligned) { return aligned && bm == 256; }
 
 // ALIGNED: x and W start on 16-byte boundaries and their pitches are multiples of 8 elements.
 // Otherwise the panels pass through registers, one step ahead of the products (S is 2 then).
@@ -265,9 +371,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
     constexpr int TM = WM / 16, TN = WN / 16;
     constexpr int NW = BN / 8 / WAVES, NI = NW + BM / 8 / WAVES;  // requests of a wave per step: weights, then positions
-    constexpr int STAGE = (BM + BN) * kStepBytes;
-    constexpr bool TURNS = ALIGNED && BM == 256 && BN == 256;
-    static_assert(!TURNS || (WAVES == 8 && S == 2 && TM == 8 && TN == 4), "the schedule of the waves that take turns");
+    constexpr int STAGE = (BM + BN) * kStepBytes;  // of the ring: weight rows, then positions
+    constexpr bool TURNS = takes_turns(BM, ALIGNED);
+    static_assert(!TURNS || (BN == 256 && WAVES == 8 && S == 2 && TM == 8 && TN == 4), "the schedule of the waves that take turns");
     static_assert(BN / 8 % WAVES == 0 && BM / 8 % WAVES == 0 && TN % 2 == 0 && BM % 16 == 0 && (ALIGNED || S == 2), "tile");
     extern __shared__ char ring[];
 
@@ -388,8 +494,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         // each ended by a barrier; waves 4..7 run one barrier behind waves 0..3, so that one wave
         // of a SIMD fetches while the other multiplies. A part's LDS reads have landed when its
         // barrier opens, so the region they came from is asked for again, for two steps later, one
-        // fetch part on; a part waits for what the next one reads. Requests are therefore up to
-        // 14 deep per wave (112 KB of a CU's 128 KB of panels).
+        // fetch part on; a part waits for what the next one reads, by the number of the wave's
+        // younger requests. Up to 14 are under way per wave, 112 KB of a CU's 128 KB of panels.
+        // (A third stage of weights in the 32 KB that are left: 2 % slower.)
         u32x4_t wf[2][2][2], xf[4][2];  // [half of the weight rows][tile][columns 32h..], [tile][columns]
         auto read_w = [&](int stage, auto half) __attribute__((always_inline)) {
             const char* wp = ring + stage * STAGE + (wave_n * WN + half * (WN / 2)) * kStepBytes;
@@ -424,10 +531,11 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             bare_barrier();
             __builtin_amdgcn_sched_barrier(0);
         };
+        constexpr std::false_type kept{};
         if (t.count > BM / 2) {
-            if (full > 0) request(0, 0, C<0>{}, C<8>{}, std::false_type{});
+            if (full > 0) request(0, 0, C<0>{}, C<8>{}, kept);
             if (full > 1) {
-                request(1, 1, C<0>{}, C<8>{}, std::false_type{});
+                request(1, 1, C<0>{}, C<8>{}, kept);
                 wait_requests<12>();
             } else {
                 wait_requests<0>();
@@ -442,25 +550,25 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                 if (more) wait_requests<10>();
                 else wait_requests<0>();
                 quarter(C<0>{}, C<0>{});
-                if (more) request(s + 2, b, C<0>{}, C<4>{}, std::false_type{});
+                if (more) request(s + 2, b, C<0>{}, C<4>{}, kept);
                 read_w(b, C<1>{});
                 if (more) wait_requests<12>();
                 else wait_requests<0>();
                 quarter(C<1>{}, C<0>{});
-                if (more) request(s + 2, b, C<4>{}, C<2>{}, std::false_type{});
+                if (more) request(s + 2, b, C<4>{}, C<2>{}, kept);
                 read_x(b, C<1>{});
                 wait_reads();
                 quarter(C<1>{}, C<1>{});
-                if (more) request(s + 2, b, C<6>{}, C<2>{}, std::false_type{});
+                if (more) request(s + 2, b, C<6>{}, C<2>{}, kept);
                 if (more) wait_requests<12>();
                 else wait_requests<0>();
                 quarter(C<0>{}, C<1>{});
             }
         } else {
             // no second half of positions: two quarters and six requests a step
-            if (full > 0) request(0, 0, C<0>{}, C<6>{}, std::false_type{});
+            if (full > 0) request(0, 0, C<0>{}, C<6>{}, kept);
             if (full > 1) {
-                request(1, 1, C<0>{}, C<4>{}, std::false_type{});
+                request(1, 1, C<0>{}, C<4>{}, kept);
                 wait_requests<6>();
             } else {
                 wait_requests<0>();
@@ -469,13 +577,13 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             if (wave >= 4) bare_barrier();
             for (int s = 0; s < full; ++s) {
                 const int b = s & 1;
-                if (s + 1 < full) request(s + 1, b ^ 1, C<4>{}, C<2>{}, std::false_type{});
+                if (s + 1 < full) request(s + 1, b ^ 1, C<4>{}, C<2>{}, kept);
                 read_w(b, C<0>{});
                 read_x(b, C<0>{});
                 if (s + 1 < full) wait_requests<6>();
                 else wait_requests<0>();
                 quarter(C<0>{}, C<0>{});
-                if (s + 2 < full) request(s + 2, b, C<0>{}, C<4>{}, std::false_type{});
+                if (s + 2 < full) request(s + 2, b, C<0>{}, C<4>{}, kept);
                 read_w(b, C<1>{});
                 if (s + 2 < full) wait_requests<6>();
                 else wait_requests<0>();
@@ -536,22 +644,75 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     wait_reads();
     bare_barrier();
     float4_t* turned = reinterpret_cast<float4_t*>(ring + wave * SHARE);
-    const int row_units = a.pair ? UNITS / 2 : UNITS;
-    const int turn_u = lane & (row_units - 1);
-    const int turn_rows = 64 / row_units;
-    const int o = n0 + wave_n * (row_units * 4) + turn_u * 4;
-    const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    // the biases of a lane's four outputs are the same for every position
-    float4_t bias[2] = {zero, zero};
+    auto finish = [&](auto chunk, auto pair) __attribute__((always_inline)) {
+        constexpr int ROW = pair ? UNITS / 2 : UNITS;  // lanes of a position, four outputs each
+        constexpr int STEP = 64 / ROW;                 // positions a wave finishes at once
+        constexpr int EACH = CHUNK / STEP < 4 ? CHUNK / STEP : 4;  // of them in a row, to overlap their loads
+        const int turn_u = lane % ROW;
+        const int o = n0 + wave_n * (ROW * 4) + turn_u * 4;
+        const int from = position_of(wave_m * WM + chunk * CHUNK);
+        const int live = o < a.n ? t.count - from : 0;
+        const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        float4_t bias[2] = {zero, zero};  // the same for every position
+        if (a.mode != kProductPartial && o < a.n) {
+            const size_t at = static_cast<size_t>(t.expert) * a.n + o;
+            if (a.bias[0] != nullptr) bias[0] = load_narrow<T>(a.bias[0] + at, false, o, a.n);
+            if (pair && a.bias[1] != nullptr) bias[1] = load_narrow<T>(a.bias[1] + at, false, o, a.n);
+        }
+#pragma unroll 1
+        for (int r0 = lane / ROW; r0 - lane / ROW < CHUNK; r0 += EACH * STEP) {
+            float4_t g[EACH], u[EACH], res[EACH];
+            float scale[EACH];
+            long draw[EACH];
+            bool ok[EACH];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        if (a.bias[m] == nullptr || a.mode == kProductPartial) continue;
+            for (int k = 0; k < EACH; ++k) {
+                const int r = r0 + k * STEP, p = t.first + from + r;
+                g[k] = turned[r * UNITS + (turn_u ^ (r & (UNITS - 1)))];
+                u[k] = pair ? turned[r * UNITS + ((turn_u + UNITS / 2) ^ (r & (UNITS - 1)))] : zero;
+                ok[k] = r < live;
+                if (a.mode == kProductDraws && ok[k]) {
+                    draw[k] = a.draws[p];
+                    ok[k] = draw[k] >= 0 && draw[k] < a.draw_count;
+                    scale[k] = ok[k] ? a.draw_weights[draw[k]] : 0.0f;
+                }
+                if (a.rows != nullptr && ok[k]) ok[k] = a.rows[p] >= 0 && a.rows[p] < a.x_rows;
+                res[k] = zero;
+                if (a.residual != nullptr && ok[k])
+                    res[k] = load_narrow<T>(a.residual + p * a.residual_stride + o, a.vec_out, o, a.n);
+            }
+            if (a.mode == kProductPartial) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (o + q < a.n) bias[m][q] = T::widen(a.bias[m][static_cast<size_t>(t.expert) * a.n + o + q]);
-    }
+                for (int k = 0; k < EACH; ++k) {
+                    if (!ok[k]) continue;
+                    const size_t p = t.first + from + r0 + k * STEP;
+                    float* dst = a.wide + (static_cast<size_t>(blockIdx.y) * (a.pair + 1) * a.positions + p) * a.n + o;
+                    store_wide(dst, g[k], o, a.n);
+                    if (pair) store_wide(dst + static_cast<size_t>(a.positions) * a.n, u[k], o, a.n);
+                }
+            } else if (a.mode == kProductDraws) {
 #pragma unroll
-    for (int chunk = 0; chunk < WM / CHUNK; ++chunk) {
+                for (int k = 0; k < EACH; ++k)
+                    if (ok[k]) store_wide(a.wide + static_cast<size_t>(draw[k]) * a.n + o, (g[k] + bias[0]) * scale[k], o, a.n);
+            } else {
+                float y[EACH * 4], up[EACH * 4];
+#pragma unroll
+                for (int k = 0; k < EACH * 4; ++k) {
+                    y[k] = g[k / 4][k % 4] + bias[0][k % 4];
+                    up[k] = u[k / 4][k % 4] + bias[1][k % 4];
+                }
+                activate(a.activation, y, up, a.limit);
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) {
+                    if (!ok[k]) continue;
+                    const int p = t.first + from + r0 + k * STEP;
+                    store_narrow<T>(a.y + p * a.y_stride + o,
+                                    float4_t{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]} + res[k], a.vec_out, o, a.n);
+                }
+            }
+        }
+    };
+    auto chunks = [&](auto chunk) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < CHUNK / 16; ++j) {
             const int r = j * 16 + (lane & 15);
@@ -561,39 +722,12 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             }
         }
         asm volatile("" ::: "memory");  // LDS serves a wave's accesses in order
-        const int from = position_of(wave_m * WM + chunk * CHUNK);
-        const int live = t.count - from;
-#pragma unroll 1
-        for (int r = lane / row_units; r < CHUNK && r < live; r += turn_rows) {
-            if (o >= a.n) break;
-            const int p = t.first + from + r;
-            float4_t g = turned[r * UNITS + (turn_u ^ (r & (UNITS - 1)))];
-            float4_t u = zero;
-            if (a.pair) u = turned[r * UNITS + ((turn_u + UNITS / 2) ^ (r & (UNITS - 1)))];
-            if (a.mode == kProductPartial) {
-                float* dst = a.wide + (static_cast<size_t>(blockIdx.y) * (a.pair + 1) * a.positions + p) * a.n + o;
-                store_wide(dst, g, o, a.n);
-                if (a.pair) store_wide(dst + static_cast<size_t>(a.positions) * a.n, u, o, a.n);
-                continue;
-            }
-            g += bias[0];
-            u += bias[1];
-            if (a.mode == kProductDraws) {
-                const long draw = a.draws[p];
-                if (draw < 0 || draw >= a.draw_count) continue;
-                store_wide(a.wide + static_cast<size_t>(draw) * a.n + o, g * a.draw_weights[draw], o, a.n);
-                continue;
-            }
-            if (a.rows != nullptr) {
-                const int row = a.rows[p];
-                if (row < 0 || row >= a.x_rows) continue;
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) g[q] = activate(a.activation, g[q], u[q], a.limit);
-            finish<T>(a, p, o, g);
-        }
+        if (a.pair) finish(chunk, std::true_type{});
+        else finish(chunk, std::false_type{});
         asm volatile("" ::: "memory");
-    }
+    };
+    chunks(C<0>{});
+    if constexpr (WM / CHUNK > 1) chunks(C<1>{});
 }
 
 // ---- a few positions: one pass of the weights through registers ------------------------------------
@@ -710,7 +844,9 @@ __device__ __forceinline__ void few_body(const ProductArgs& a, const ProductTile
         const int row = a.rows[p];
         if (row < 0 || row >= a.x_rows) return;
     }
-    float y = activate(a.activation, g, MATS == 2 ? total(1) : 0.0f, a.limit);
+    float value[1] = {g}, up[1] = {MATS == 2 ? total(1) : 0.0f};
+    activate(a.activation, value, up, a.limit);
+    float y = value[0];
     if (a.residual != nullptr) y += T::widen(a.residual[p * a.residual_stride + o]);
     a.y[p * a.y_stride + o] = T::round(y);
 }
@@ -867,17 +1003,16 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, 
             }
         }
     }
-    float4_t y;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        float g = v[0][q], u = v[1][q];
-        if (o + q < a.n) {
-            if (a.bias[0] != nullptr) g += T::widen(a.bias[0][o + q]);
-            if (a.bias[1] != nullptr) u += T::widen(a.bias[1][o + q]);
-        }
-        y[q] = activate(a.activation, g, u, a.limit);
+        if (o + q >= a.n) break;
+        if (a.bias[0] != nullptr) v[0][q] += T::widen(a.bias[0][o + q]);
+        if (a.bias[1] != nullptr) v[1][q] += T::widen(a.bias[1][o + q]);
     }
-    finish<T>(a, p, o, y);
+    activate(a.activation, v[0], v[1], a.limit);
+    float4_t y = {v[0][0], v[0][1], v[0][2], v[0][3]};
+    if (a.residual != nullptr) y += load_narrow<T>(a.residual + p * a.residual_stride + o, a.vec_out, o, a.n);
+    store_narrow<T>(a.y + p * a.y_stride + o, y, a.vec_out, o, a.n);
 }
 
 // out[t][i] = round(base[t][i] + sum of the token's contributions in slot order). A draw whose id
@@ -920,6 +1055,16 @@ __global__ __launch_bounds__(256) void product_combine_kernel(const float* __res
 
 // ---- launches --------------------------------------------------------------------------------
 
+constexpr int kTurnsTile = 256;
+
+// Entries of the tile table: an XCD's run is an eighth of the cost, which is that many tiles if every
+// one of them costs half.
+static long table_entries(int n, bool pair, int experts, int positions) {
+    const long row_blocks = (n * (pair ? 2L : 1L) + kTurnsTile - 1) / kTurnsTile;
+    const long lists = experts < positions ? experts : positions;
+    return ((positions / (kTurnsTile / 2) + lists) * row_blocks / kXcds + 2) * kXcds;
+}
+
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N, int S, bool ALIGNED>
 static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
     auto kernel = product_kernel<T, BM, BN, WAVES_M, WAVES_N, S, ALIGNED>;
@@ -942,9 +1087,18 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
     long windows = (static_cast<long>(a.positions) + BM - 1) / BM;
     if (a.offsets != nullptr) windows = a.positions / BM + (a.experts < a.positions ? a.experts : a.positions);
     long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
-    if (BM == 256 && ALIGNED) grid += kXcds * (kXcdCus / 2);  // room for a last round in halves
+    if (BM == kTurnsTile && ALIGNED) {
+        if (a.offsets == nullptr) grid += kXcds * (kXcdCus / 2);  // room for a last round in halves
+        else grid = table_entries(a.n, a.pair, a.experts, a.positions);
+    }
     AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
-    kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(a);
+    ProductArgs args = a;
+    if (BM == kTurnsTile && ALIGNED && a.offsets != nullptr) {
+        product_tiles_kernel<<<1, 1024, 0, stream>>>(a, BM, static_cast<int>(row_blocks), static_cast<int>(grid), a.table);
+        AEON_LAUNCH_CHECK();
+        args.tiles = a.table;
+    }
+    kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(args);
     AEON_LAUNCH_CHECK();
     return AEON_OK;
 }
@@ -1090,6 +1244,24 @@ static bool combine_direct(const aeon_projection& w, int tokens, int slots) {
     return tokens <= kDirectTokens && static_cast<long>(tokens) * slots <= kDirectDraws && w.in_dim >= kFewColumns;
 }
 
+// Bytes of the tile table a product over lists needs.
+static size_t table_bytes(const aeon_projection& w, int experts, int positions) {
+    if (positions <= 0 || experts <= 0 || plan_experts(w, positions, experts) != kTurnsTile) return 0;
+    return static_cast<size_t>(table_entries(w.out_dim, w.activation == AEON_ACT_SWIGLU, experts, positions)) * sizeof(int4);
+}
+
+static size_t contrib_bytes(const aeon_projection& w, int tokens, int slots) {
+    const size_t bytes = static_cast<size_t>(tokens) * slots * w.out_dim * sizeof(float);
+    return (bytes + 15) / 16 * 16;
+}
+
+static int check_workspace(const void* d_workspace, size_t bytes, size_t need, const char* who) {
+    AEON_REQUIRE(bytes >= need && (need == 0 || (d_workspace != nullptr && on_boundary(d_workspace, 16))),
+                 AEON_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes on a 16-byte boundary (%zu given)", who, need,
+                 bytes);
+    return AEON_OK;
+}
+
 static size_t linear_workspace(const aeon_projection& w, int tokens, const ProductPlan& p) {
     if (p.splits == 1) return 0;
     return static_cast<size_t>(p.splits) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1) * tokens * w.out_dim * sizeof(float);
@@ -1124,9 +1296,7 @@ extern "C" int aeon_linear(const aeon_projection* projection, const void* d_x, l
                  "%s: an output on the residual needs the residual's row pitch", who);
     const ProductPlan plan = plan_linear(w, tokens);
     const size_t need = linear_workspace(w, tokens, plan);
-    AEON_REQUIRE(workspace_bytes >= need && (need == 0 || (d_workspace != nullptr && on_boundary(d_workspace, 16))),
-                 AEON_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes on a 16-byte boundary (%zu given)", who, need,
-                 workspace_bytes);
+    if (int rc = check_workspace(d_workspace, workspace_bytes, need, who)) return rc;
     ProductArgs a = projection_args(w);
     a.x = static_cast<const uint16_t*>(d_x);
     a.x_stride = x_stride;
@@ -1149,10 +1319,15 @@ extern "C" int aeon_linear(const aeon_projection* projection, const void* d_x, l
     return AEON_OK;
 }
 
+extern "C" size_t aeon_expert_linear_workspace_bytes(const aeon_projection* projection, int experts, int positions) {
+    if (check_projection(projection, "aeon_expert_linear_workspace_bytes") != AEON_OK) return 0;
+    return table_bytes(*projection, experts, positions);
+}
+
 extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,
                                   const void* d_x, long x_stride, int x_rows, const int32_t* d_expert_offsets,
                                   const int32_t* d_row_indices, int positions, void* d_y, long y_stride,
-                                  void* stream) {
+                                  void* d_workspace, size_t workspace_bytes, void* stream) {
     const char* who = "aeon_expert_linear";
     if (int rc = check_projection(projection, who)) return rc;
     const aeon_projection& w = *projection;
@@ -1167,7 +1342,9 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
                  who, x_stride, y_stride);
     AEON_REQUIRE(d_y != d_x && d_y != w.d_weight && d_y != w.d_weight_up, AEON_ERR_INVALID_ARGUMENT,
                  "%s: the output must not alias the activations or the weights", who);
+    if (int rc = check_workspace(d_workspace, workspace_bytes, table_bytes(w, experts, positions), who)) return rc;
     ProductArgs a = projection_args(w);
+    a.table = static_cast<int4*>(d_workspace);
     a.expert_stride = expert_stride;
     a.x = static_cast<const uint16_t*>(d_x);
     a.x_stride = x_stride;
@@ -1181,10 +1358,11 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
     return launch_product(w.dtype, plan_experts(w, positions, experts), a, 1, as_stream(stream));
 }
 
-extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots) {
-    if (check_projection(projection, "aeon_expert_combine_workspace_bytes") != AEON_OK || tokens <= 0 || slots <= 0) return 0;
-    if (combine_direct(*projection, tokens, slots)) return 0;
-    return static_cast<size_t>(tokens) * slots * projection->out_dim * sizeof(float);
+extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int experts, int tokens, int slots) {
+    if (check_projection(projection, "aeon_expert_combine_workspace_bytes") != AEON_OK || tokens <= 0 || slots <= 0 ||
+        static_cast<long>(tokens) * slots > 0x7fffffffL || combine_direct(*projection, tokens, slots))
+        return 0;
+    return contrib_bytes(*projection, tokens, slots) + table_bytes(*projection, experts, tokens * slots);
 }
 
 extern "C" int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,
@@ -1212,9 +1390,8 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
                  "%s: the output must not alias the hidden rows or the weights", who);
     AEON_REQUIRE(d_out != d_base || out_stride == base_stride, AEON_ERR_INVALID_ARGUMENT,
                  "%s: an output on the base needs the base's row pitch", who);
-    const size_t need = aeon_expert_combine_workspace_bytes(projection, tokens, slots);
-    AEON_REQUIRE(workspace_bytes >= need && (need == 0 || (d_workspace != nullptr && on_boundary(d_workspace, 16))),
-                 AEON_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes on a 16-byte boundary (%zu given)", who, need, workspace_bytes);
+    const size_t need = aeon_expert_combine_workspace_bytes(projection, experts, tokens, slots);
+    if (int rc = check_workspace(d_workspace, workspace_bytes, need, who)) return rc;
     ProductArgs a = projection_args(w);
     a.expert_stride = expert_stride;
     a.x = static_cast<const uint16_t*>(d_h);
@@ -1225,6 +1402,7 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
     a.positions = tokens * slots;
     a.mode = kProductDraws;
     a.wide = static_cast<float*>(d_workspace);
+    a.table = reinterpret_cast<int4*>(static_cast<char*>(d_workspace) + contrib_bytes(w, tokens, slots));
     a.draws = d_draw_indices;
     a.draw_weights = d_topk_weights;
     a.draw_count = tokens * slots;
