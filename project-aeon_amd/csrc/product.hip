@@ -324,23 +324,34 @@ __device__ __forceinline__ u32x4_t load_columns(const uint16_t* p, int c, int k)
     return __builtin_bit_cast(u32x4_t, v);
 }
 
-__device__ __forceinline__ void store_wide(float* dst, const float4_t& v, int o, int n) {
-    if (n % 4 == 0) {
-        *reinterpret_cast<float4_t*>(dst) = v;
+// Four outputs o .. o+3 of a row of n, fp32 or one 16-bit type, at any element's alignment (global
+// memory takes that); the ones past the row's end are zeros, or not written.
+__device__ __forceinline__ void store_wide(float* p, const float4_t& v, int o, int n) {
+    typedef float4_t __attribute__((aligned(4))) loose_t;
+    if (o + 4 <= n) {
+        *reinterpret_cast<loose_t*>(p) = v;
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (o + q < n) dst[q] = v[q];
+            if (o + q < n) p[q] = v[q];
     }
 }
-
-// Four values of one 16-bit type from p on, zeros past the row's end.
-template <class T>
-__device__ __forceinline__ float4_t load_narrow(const uint16_t* p, bool vec, int o, int n) {
+__device__ __forceinline__ float4_t load_wide(const float* p, int o, int n) {
+    typedef float4_t __attribute__((aligned(4))) loose_t;
+    if (o + 4 <= n) return __builtin_nontemporal_load(reinterpret_cast<const loose_t*>(p));
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (vec) {
-        const uint2 r = *reinterpret_cast<const uint2*>(p);
-        v = float4_t{T::widen(r.x & 0xFFFFu), T::widen(r.x >> 16), T::widen(r.y & 0xFFFFu), T::widen(r.y >> 16)};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (o + q < n) v[q] = p[q];
+    return v;
+}
+template <class T>
+__device__ __forceinline__ float4_t load_narrow(const uint16_t* p, int o, int n) {
+    typedef u32x2_t __attribute__((aligned(2))) loose_t;
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (o + 4 <= n) {
+        const u32x2_t r = *reinterpret_cast<const loose_t*>(p);
+        v = float4_t{T::widen(r[0] & 0xFFFFu), T::widen(r[0] >> 16), T::widen(r[1] & 0xFFFFu), T::widen(r[1] >> 16)};
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -350,9 +361,10 @@ __device__ __forceinline__ float4_t load_narrow(const uint16_t* p, bool vec, int
 }
 // The one rounding.
 template <class T>
-__device__ __forceinline__ void store_narrow(uint16_t* p, const float4_t& v, bool vec, int o, int n) {
-    if (vec) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(T::round2(v[0], v[1]), T::round2(v[2], v[3]));
+__device__ __forceinline__ void store_narrow(uint16_t* p, const float4_t& v, int o, int n) {
+    typedef u32x2_t __attribute__((aligned(2))) loose_t;
+    if (o + 4 <= n) {
+        *reinterpret_cast<loose_t*>(p) = u32x2_t{T::round2(v[0], v[1]), T::round2(v[2], v[3])};
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -471,21 +483,27 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             *reinterpret_cast<u32x4_t*>(ring + stage * STAGE + panel_row(i) * kStepBytes + lane * 16) = held[i];
     };
     const int frag = (lane & 15) * kStepBytes + (((lane >> 4) ^ (lane & 7)) * 16);
-    auto multiply = [&](int stage) __attribute__((always_inline)) {
+    struct Fragments {
+        u32x4_t w[2][TN], x[2][TM];  // [columns 32h ..][tile]
+    };
+    auto read_step = [&](Fragments& f, int stage) __attribute__((always_inline)) {
         const char* wp = ring + stage * STAGE + wave_n * WN * kStepBytes;
         const char* xp = ring + stage * STAGE + (BN + wave_m * WM) * kStepBytes;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            u32x4_t wf[TN], xf[TM];
 #pragma unroll
-            for (int i = 0; i < TN; ++i) wf[i] = *reinterpret_cast<const u32x4_t*>(wp + i * 2048 + (frag ^ (h * 64)));
+            for (int i = 0; i < TN; ++i) f.w[h][i] = *reinterpret_cast<const u32x4_t*>(wp + i * 2048 + (frag ^ (h * 64)));
 #pragma unroll
-            for (int j = 0; j < TM; ++j) xf[j] = *reinterpret_cast<const u32x4_t*>(xp + j * 2048 + (frag ^ (h * 64)));
+            for (int j = 0; j < TM; ++j) f.x[h][j] = *reinterpret_cast<const u32x4_t*>(xp + j * 2048 + (frag ^ (h * 64)));
+        }
+    };
+    auto multiply = [&](const Fragments& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < TN; ++i)
 #pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = T::mfma(wf[i], xf[j], acc[i][j]);
-        }
+                for (int j = 0; j < TM; ++j) acc[i][j] = T::mfma(f.w[h][i], f.x[h][j], acc[i][j]);
     };
 
     if constexpr (TURNS) {
@@ -514,18 +532,23 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                 for (int h = 0; h < 2; ++h)
                     xf[j][h] = *reinterpret_cast<const u32x4_t*>(xp + j * 2048 + (frag ^ (h * 64)));
         };
-        auto quarter = [&](auto wh, auto xh) __attribute__((always_inline)) {
+        // products of weight half `first` (and, in a whole part, the other half after it) with position half xh
+        auto part = [&](auto first, auto both, auto xh) __attribute__((always_inline)) {
             __builtin_amdgcn_sched_barrier(0);
             bare_barrier();
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int w = 0; w <= both; ++w) {
+                const int wh = w == 0 ? first : 1 - first;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[wh * 2 + i][xh * 4 + j] = T::mfma(wf[wh][i][h], xf[j][h], acc[wh * 2 + i][xh * 4 + j]);
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[wh * 2 + i][xh * 4 + j] = T::mfma(wf[wh][i][h], xf[j][h], acc[wh * 2 + i][xh * 4 + j]);
+            }
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             bare_barrier();
@@ -535,8 +558,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         if (t.count > BM / 2) {
             if (full > 0) request(0, 0, C<0>{}, C<8>{}, kept);
             if (full > 1) {
-                request(1, 1, C<0>{}, C<8>{}, kept);
-                wait_requests<12>();
+                request(1, 1, C<0>{}, C<6>{}, kept);
+                wait_requests<8>();
             } else {
                 wait_requests<0>();
             }
@@ -544,25 +567,18 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
             if (wave >= 4) bare_barrier();
             for (int s = 0; s < full; ++s) {
                 const int b = s & 1;
-                const bool more = s + 2 < full;
+                if (s + 1 < full) request(s + 1, b ^ 1, C<6>{}, C<2>{}, kept);
                 read_w(b, C<0>{});
                 read_x(b, C<0>{});
-                if (more) wait_requests<10>();
-                else wait_requests<0>();
-                quarter(C<0>{}, C<0>{});
-                if (more) request(s + 2, b, C<0>{}, C<4>{}, kept);
                 read_w(b, C<1>{});
-                if (more) wait_requests<12>();
+                if (s + 1 < full) wait_requests<8>();  // the second positions of this step
                 else wait_requests<0>();
-                quarter(C<1>{}, C<0>{});
-                if (more) request(s + 2, b, C<4>{}, C<2>{}, kept);
+                part(C<0>{}, C<1>{}, C<0>{});
+                if (s + 2 < full) request(s + 2, b, C<0>{}, C<6>{}, kept);
                 read_x(b, C<1>{});
-                wait_reads();
-                quarter(C<1>{}, C<1>{});
-                if (more) request(s + 2, b, C<6>{}, C<2>{}, kept);
-                if (more) wait_requests<12>();
+                if (s + 2 < full) wait_requests<8>();  // the next step's weights and first positions
                 else wait_requests<0>();
-                quarter(C<0>{}, C<1>{});
+                part(C<1>{}, C<1>{}, C<1>{});
             }
         } else {
             // no second half of positions: two quarters and six requests a step
@@ -582,54 +598,77 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                 read_x(b, C<0>{});
                 if (s + 1 < full) wait_requests<6>();
                 else wait_requests<0>();
-                quarter(C<0>{}, C<0>{});
+                part(C<0>{}, C<0>{}, C<0>{});
                 if (s + 2 < full) request(s + 2, b, C<0>{}, C<4>{}, kept);
                 read_w(b, C<1>{});
                 if (s + 2 < full) wait_requests<6>();
                 else wait_requests<0>();
-                quarter(C<1>{}, C<0>{});
+                part(C<1>{}, C<0>{}, C<0>{});
             }
         }
         if (wave < 4) bare_barrier();
     } else if constexpr (ALIGNED) {
+        // A step's fragments are read while the step before is multiplied; its stage is asked for
+        // again, for S steps later, behind the barrier that follows the reads.
         auto ring_loop = [&](auto stream) __attribute__((always_inline)) {
 #pragma unroll
-            for (int s = 0; s < S - 1; ++s) {
+            for (int s = 0; s < S; ++s) {
                 if (s < full) request(s, s, C<0>{}, C<NI>{}, stream);
             }
-            int stage = 0, ahead = S - 1;
-            for (int s = 0; s < full; ++s) {
-                if (s + S - 2 < full) wait_requests<(S - 2) * NI>();  // the S-2 younger steps may be under way
+            Fragments f[2];
+            if (S <= full) wait_requests<(S - 1) * NI>();
+            else wait_requests<0>();
+            bare_barrier();
+            if (full > 0) read_step(f[0], 0);
+            int stage = 0;
+            auto step = [&](int s, const Fragments& now, Fragments& next) __attribute__((always_inline)) {
+                if (s + S - 1 < full) wait_requests<(S - 2) * NI>();  // step s+1 is there, S-2 younger ones are under way
                 else wait_requests<0>();
                 bare_barrier();
-                if (s + S - 1 < full) request(s + S - 1, ahead, C<0>{}, C<NI>{}, stream);
-                multiply(stage);
+                if (s + S < full) request(s + S, stage, C<0>{}, C<NI>{}, stream);
                 stage = stage + 1 == S ? 0 : stage + 1;
-                ahead = ahead + 1 == S ? 0 : ahead + 1;
+                if (s + 1 < full) read_step(next, stage);
+                multiply(now);
+            };
+            for (int s = 0; s < full; s += 2) {
+                step(s, f[0], f[1]);
+                if (s + 1 < full) step(s + 1, f[1], f[0]);
             }
         };
         if (t.only) ring_loop(std::true_type{});
         else ring_loop(std::false_type{});
     } else {
-        if (steps > 0) {
-            fetch(0);
-            put(0);
-        }
-        for (int s = 0; s < steps; ++s) {
+        // the same through registers: loads two steps ahead of the products, LDS one
+        Fragments f[2];
+        fetch(0);
+        put(0);
+        if (steps > 1) fetch(1);
+        __syncthreads();
+        read_step(f[0], 0);
+        if (steps > 1) put(1);
+        if (steps > 2) fetch(2);
+        auto step = [&](int s, const Fragments& now, Fragments& next) __attribute__((always_inline)) {
             __syncthreads();
-            if (s + 1 < steps) fetch(s + 1);
-            multiply(s & 1);
-            if (s + 1 < steps) put((s + 1) & 1);
+            if (s + 1 < steps) read_step(next, (s + 1) & 1);
+            multiply(now);
+            if (s + 2 < steps) put(s & 1);
+            if (s + 3 < steps) fetch(s + 3);
+        };
+        for (int s = 0; s < steps; s += 2) {
+            step(s, f[0], f[1]);
+            if (s + 1 < steps) step(s + 1, f[1], f[0]);
         }
     }
     if (ALIGNED && steps > full) {  // the last columns of a K that is no multiple of 64
+        Fragments f;
         fetch(full);
         wait_reads();
         bare_barrier();
         put(0);
         wait_reads();
         bare_barrier();
-        multiply(0);
+        read_step(f, 0);
+        multiply(f);
     }
 
     // Epilogue. A lane holds outputs 4*(lane/16) .. +3 of a 16-row tile for position lane%16; the tile
@@ -656,8 +695,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         float4_t bias[2] = {zero, zero};  // the same for every position
         if (a.mode != kProductPartial && o < a.n) {
             const size_t at = static_cast<size_t>(t.expert) * a.n + o;
-            if (a.bias[0] != nullptr) bias[0] = load_narrow<T>(a.bias[0] + at, false, o, a.n);
-            if (pair && a.bias[1] != nullptr) bias[1] = load_narrow<T>(a.bias[1] + at, false, o, a.n);
+            if (a.bias[0] != nullptr) bias[0] = load_narrow<T>(a.bias[0] + at, o, a.n);
+            if (pair && a.bias[1] != nullptr) bias[1] = load_narrow<T>(a.bias[1] + at, o, a.n);
         }
 #pragma unroll 1
         for (int r0 = lane / ROW; r0 - lane / ROW < CHUNK; r0 += EACH * STEP) {
@@ -679,7 +718,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                 if (a.rows != nullptr && ok[k]) ok[k] = a.rows[p] >= 0 && a.rows[p] < a.x_rows;
                 res[k] = zero;
                 if (a.residual != nullptr && ok[k])
-                    res[k] = load_narrow<T>(a.residual + p * a.residual_stride + o, a.vec_out, o, a.n);
+                    res[k] = load_narrow<T>(a.residual + p * a.residual_stride + o, o, a.n);
             }
             if (a.mode == kProductPartial) {
 #pragma unroll
@@ -707,7 +746,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                     if (!ok[k]) continue;
                     const int p = t.first + from + r0 + k * STEP;
                     store_narrow<T>(a.y + p * a.y_stride + o,
-                                    float4_t{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]} + res[k], a.vec_out, o, a.n);
+                                    float4_t{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]} + res[k], o, a.n);
                 }
             }
         }
@@ -986,33 +1025,25 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, 
     const int p = static_cast<int>(at / groups);
     const int o = static_cast<int>(at - static_cast<long>(p) * groups) * 4;
     const int mats = a.pair + 1;
-    float v[2][4] = {};
+    float4_t sum[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    const size_t share = static_cast<size_t>(a.positions) * a.n;
     for (int s = 0; s < splits; ++s) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            if (m >= mats) break;
-            const float* src = a.wide + ((static_cast<size_t>(s) * mats + m) * a.positions + p) * a.n + o;
-            if (a.n % 4 == 0) {
-                const float4_t w = *reinterpret_cast<const float4_t*>(src);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) v[m][q] += w[q];
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (o + q < a.n) v[m][q] += src[q];
-            }
-        }
+        const float* src = a.wide + static_cast<size_t>(s) * mats * share + static_cast<size_t>(p) * a.n + o;
+        sum[0] += load_wide(src, o, a.n);
+        if (a.pair) sum[1] += load_wide(src + share, o, a.n);
     }
+    float v[4], u[4];
+    if (a.bias[0] != nullptr) sum[0] += load_narrow<T>(a.bias[0] + o, o, a.n);
+    if (a.bias[1] != nullptr) sum[1] += load_narrow<T>(a.bias[1] + o, o, a.n);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        if (o + q >= a.n) break;
-        if (a.bias[0] != nullptr) v[0][q] += T::widen(a.bias[0][o + q]);
-        if (a.bias[1] != nullptr) v[1][q] += T::widen(a.bias[1][o + q]);
+        v[q] = sum[0][q];
+        u[q] = sum[1][q];
     }
-    activate(a.activation, v[0], v[1], a.limit);
-    float4_t y = {v[0][0], v[0][1], v[0][2], v[0][3]};
-    if (a.residual != nullptr) y += load_narrow<T>(a.residual + p * a.residual_stride + o, a.vec_out, o, a.n);
-    store_narrow<T>(a.y + p * a.y_stride + o, y, a.vec_out, o, a.n);
+    activate(a.activation, v, u, a.limit);
+    float4_t y = {v[0], v[1], v[2], v[3]};
+    if (a.residual != nullptr) y += load_narrow<T>(a.residual + p * a.residual_stride + o, o, a.n);
+    store_narrow<T>(a.y + p * a.y_stride + o, y, o, a.n);
 }
 
 // out[t][i] = round(base[t][i] + sum of the token's contributions in slot order). A draw whose id
@@ -1027,30 +1058,14 @@ __global__ __launch_bounds__(256) void product_combine_kernel(const float* __res
     if (at >= static_cast<long>(tokens) * groups) return;
     const int t = static_cast<int>(at / groups);
     const int o = static_cast<int>(at - static_cast<long>(t) * groups) * 4;
-    float v[4] = {};
-    if (base != nullptr) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (o + q < n) v[q] = T::widen(base[t * base_stride + o + q]);
-    }
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (base != nullptr) v = load_narrow<T>(base + t * base_stride + o, o, n);
     for (int s = 0; s < slots; ++s) {
         const long draw = static_cast<long>(t) * slots + s;
         const int id = ids[draw];
-        if (id < 0 || id >= experts) continue;
-        const float* src = contrib + static_cast<size_t>(draw) * n + o;
-        if (n % 4 == 0) {
-            const float4_t w = __builtin_nontemporal_load(reinterpret_cast<const float4_t*>(src));
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += w[q];
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (o + q < n) v[q] += src[q];
-        }
+        if (id >= 0 && id < experts) v += load_wide(contrib + static_cast<size_t>(draw) * n + o, o, n);
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        if (o + q < n) out[t * out_stride + o + q] = T::round(v[q]);
+    store_narrow<T>(out + t * out_stride + o, v, o, n);
 }
 
 // ---- launches --------------------------------------------------------------------------------
@@ -1149,8 +1164,6 @@ static bool on_boundary(const void* p, uintptr_t bytes) { return (reinterpret_ca
 static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipStream_t stream) {
     const bool aligned = on_boundary(a.x, 16) && on_boundary(a.w[0], 16) && on_boundary(a.w[1], 16) &&
                          a.x_stride % 8 == 0 && a.w_stride % 8 == 0 && a.expert_stride % 8 == 0;
-    a.vec_out = a.n % 4 == 0 && a.y_stride % 4 == 0 && on_boundary(a.y, 8) && a.residual_stride % 4 == 0 &&
-                on_boundary(a.residual, 8);
     if (tile == kFewMax) return dtype == AEON_DTYPE_F16 ? launch_few<F16>(a, stream) : launch_few<BF16>(a, stream);
     if (dtype == AEON_DTYPE_F16) {
         return aligned ? launch_tiles<F16, true>(tile, a, splits, stream) : launch_tiles<F16, false>(tile, a, splits, stream);

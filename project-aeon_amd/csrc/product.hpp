@@ -40,7 +40,6 @@ struct ProductArgs {
     int4* table;               // room for the tile table of lists, and
     const int4* tiles;         // that table where the kernel reads one
     int split_steps;           // kProductPartial: 64-column steps of one share of K
-    int vec_out;               // y, residual and bias may be moved four values at a time
 };
 
 }  // namespace aeon355
