@@ -375,7 +375,7 @@ __device__ __forceinline__ void store_narrow(uint16_t* p, const float4_t& v, int
 // The tile that fills a CU is run by waves that take turns (below).
 constexpr bool takes_turns(int bm, bool aligned) { return aligned && bm == 256; }
 
-// ALIGNED: x and W start on 16-byte boundaries and their pitches are multiples of 8 elements.
+// ALIGNED: every row of x and W starts on a 4-byte boundary, which is what vector memory asks for.
 // Otherwise the panels pass through registers, one step ahead of the products (S is 2 then).
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N, int S, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const ProductArgs a) {
@@ -1162,8 +1162,8 @@ static int launch_tiles(int tile, const ProductArgs& a, int splits, hipStream_t 
 static bool on_boundary(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipStream_t stream) {
-    const bool aligned = on_boundary(a.x, 16) && on_boundary(a.w[0], 16) && on_boundary(a.w[1], 16) &&
-                         a.x_stride % 8 == 0 && a.w_stride % 8 == 0 && a.expert_stride % 8 == 0;
+    const bool aligned = on_boundary(a.x, 4) && on_boundary(a.w[0], 4) && on_boundary(a.w[1], 4) && a.x_stride % 2 == 0 &&
+                         a.w_stride % 2 == 0 && a.expert_stride % 2 == 0;
     if (tile == kFewMax) return dtype == AEON_DTYPE_F16 ? launch_few<F16>(a, stream) : launch_few<BF16>(a, stream);
     if (dtype == AEON_DTYPE_F16) {
         return aligned ? launch_tiles<F16, true>(tile, a, splits, stream) : launch_tiles<F16, false>(tile, a, splits, stream);
