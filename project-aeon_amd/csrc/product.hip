@@ -1176,34 +1176,73 @@ struct ProductPlan {
     int tile, splits, split_steps;
 };
 
+// What a tile costs, us: a 64-column step of a workgroup that has its CU to itself, of one of two that
+// share it, and the rest of a workgroup (launch, first requests, epilogue). Least squares over products of
+// 5 to 4096 tokens with matrices of 512 x 1024 to 7168 x 7168, each at every tile and at one to eight
+// shares, weights cold (72 products; the plan made from these figures is within 0.9 % of the best one
+// measured in the mean, and 16 % at worst).
+struct TileCost {
+    int positions, rows;
+    double step_alone, step_shared, fixed;
+};
+constexpr TileCost kTileCosts[] = {{16, 64, 0.12, 0.27, 2.8}, {32, 64, 0.16, 0.34, 3.0}, {64, 64, 0.21, 0.40, 2.9},
+                                   {128, 128, 0.68, 1.04, 4.1}, {kTurnsTile, kTurnsTile, 1.38, 0.0, 18.8}};
+
+// Every tile and number of shares priced: rounds of workgroups, the weights' way from memory, and the
+// second launch that joins shares with its traffic.
 static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
-    const bool pair = w.activation == AEON_ACT_SWIGLU;
-    const long n = static_cast<long>(w.out_dim) * (pair ? 2 : 1);
-    auto tiles = [&](long bm, long bn) { return (tokens + bm - 1) / bm * ((n + bn - 1) / bn); };
-    ProductPlan p{16, 1, 0};
     if (tokens <= kFewMax && w.in_dim >= kFewColumns) return ProductPlan{kFewMax, 1, 0};
-    if (tokens > 16) p.tile = 32;
-    if (tokens > 32) p.tile = 64;
-    if (tokens > 64 && tiles(128, 128) >= 256) p.tile = 128;
-    if (tokens > 128 && tiles(256, 256) >= 192) p.tile = 256;
+    const double n = static_cast<double>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     const int steps = (w.in_dim + kStep - 1) / kStep;
-    const long have = tiles(p.tile, p.tile <= 64 ? 64 : p.tile);
-    const long want = p.tile <= 64 ? 512 : 256;
-    long splits = want / (have > 0 ? have : 1);
-    if (splits > steps / 8) splits = steps / 8;
-    if (splits > 16) splits = 16;
-    if (splits < 1 || p.tile > 64) splits = 1;
-    p.split_steps = static_cast<int>((steps + splits - 1) / splits);
-    p.splits = (steps + p.split_steps - 1) / p.split_steps;
-    return p;
+    const double stream = (n + tokens) * w.in_dim * 2 / 9.3e6 + 2.7;
+    ProductPlan best{16, 1, steps};
+    double best_us = 0.0;
+    for (const TileCost& t : kTileCosts) {
+        if (t.positions > 64 ? t.positions > 2L * tokens : t.positions < 64 && t.positions * 4L < tokens) continue;
+        const double tiles = static_cast<double>((tokens + t.positions - 1) / t.positions) *
+                             ((static_cast<long>(n) + t.rows - 1) / t.rows);
+        for (int splits : {1, 2, 3, 4, 6, 8}) {
+            if (splits > 1 && (splits > steps / 2 || tiles * splits > 1100)) break;
+            const int each = (steps + splits - 1) / splits;
+            const long groups = static_cast<long>(tiles * splits);
+            double us;
+            if (t.positions == kTurnsTile) {
+                const long last = groups % 256;
+                const double half = 0.55;  // of a tile's products, where its positions or its last round fill one half
+                us = groups / 256 * (each * t.step_alone + t.fixed);
+                if (last > 0) us += each * t.step_alone * (last <= 128 && splits == 1 && tokens > 128 ? half : 1.0) + t.fixed;
+                if (tokens <= 128) us *= half;
+            } else {
+                const long last = groups % 512;
+                us = groups / 512 * (each * t.step_shared + t.fixed);
+                if (last > 0) us += each * (last <= 256 ? t.step_alone : t.step_shared) + t.fixed;
+            }
+            if (us < stream) us = stream;
+            if (splits > 1) us += 1.3 + 8.0 * splits * tokens * n / 11e6;
+            if (best_us == 0.0 || us < best_us) {
+                best_us = us;
+                best = ProductPlan{t.positions, splits, each};
+            }
+        }
+    }
+    best.splits = (steps + best.split_steps - 1) / best.split_steps;
+    return best;
 }
 
-// Experts: by how many positions an expert holds on average.
+// Lists: by how many positions an expert holds on average, and only as large a tile as leaves the CUs
+// enough of them (half a window an expert is taken to be short). Measured, us per product at a mean of 16 /
+// 32 / 64 / 96 / 128 / 192 positions, 64 experts of 4096 x 2048: tile 32: 172 / 222 / 317; 64: 168 / 193 /
+// 259 / 312 / 385; 128: 188 / 206 / 229 / 262 / 303 / 384; 256: 221 / 223 / 232 / 274 / 286 / 278. Eight experts of 4096 x 4096
+// at 192: tile 64 118, 128 77, 256 93; at 256: 151, 135, 99.
 static int plan_experts(const aeon_projection& w, int positions, int experts) {
     if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kFewMax;
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
-    return mean <= 8 ? 16 : mean <= 24 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
+    const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
+    auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
+    if (mean > 112 && tiles(256) >= 192) return kTurnsTile;
+    if (mean > 48 && tiles(128) >= 192) return 128;
+    return mean <= 12 ? 16 : mean <= 24 ? 32 : 64;
 }
 
 static int check_projection(const aeon_projection* w, const char* who) {

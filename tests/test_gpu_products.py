@@ -159,6 +159,35 @@ def test_linear_keeps_inf_and_nan_in_their_own_rows(tokens, k, dtype):
     assert bool(got[:, others].isfinite().all())
 
 
+# long enough for the largest tiles: a last round cut into halves and a last window of 52 positions, shares of
+# K of the two largest tiles with a partial last step, and a row pitch that is off every 4-byte boundary
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("tokens,k,n", [(2100, 4168, 8000), (400, 7170, 7100), (520, 4104, 2100), (250, 7176, 7000),
+                                        (3000, 4104, 4104), (2100, 4167, 8000)])
+def test_linear_on_the_largest_tiles_is_exact(tokens, k, n, gated, dtype):
+    """Whole numbers as above. Gated, the gate is a constant 0 + bias beyond the clamp, so that the result is
+    silu(LIMIT) times the clamped whole-number product."""
+    torch, dense = _setup()
+    dt = _dtype(torch, dtype)
+    print("linear", tokens, k, n, gated, dtype, flush=True)
+    x = _whole(torch, (tokens, k), dt, 1)
+    if not gated:
+        w, b, r = _whole(torch, (n, k), dt, 2), _whole(torch, (n,), dt, 3, 9), _whole(torch, (tokens, n), dt, 4, 9)
+        guard = torch.full((tokens + 1, n), 77.0, dtype=dt, device="cuda")
+        dense.linear(x, w, b, residual=r, out=guard[:tokens])
+        assert torch.equal(guard[:tokens], (_mm64(x, w) + b.double() + r.double()).to(dt))
+        assert bool((guard[tokens] == 77.0).all())
+        return
+    w, up = _whole(torch, (2, n // 2, k), dt, 2, 1)
+    w.zero_()
+    b = torch.full((n // 2,), 9.0, dtype=dt, device="cuda")
+    got = dense.linear(x, w, b, activation="swiglu", weight_up=up, swiglu_limit=LIMIT)
+    silu = LIMIT * torch.special.expit(torch.tensor(LIMIT, dtype=torch.float64)).item()
+    want = _mm64(x, up).clamp(-LIMIT, LIMIT) * silu
+    _near(torch, got, want, 2.0 ** -20 * want.abs())
+
+
 def _lists(torch, ids, experts):
     """What the permutation defines: draws sorted by expert, ascending inside one; ids outside are dropped."""
     flat = ids.reshape(-1).cpu().numpy()
@@ -186,7 +215,8 @@ def _ids(torch, kind, tokens, slots, experts, seed):
 
 
 EXPERT_SHAPES = [(1, 1, 1, 64, 32), (1, 8, 256, 128, 64), (3, 2, 5, 100, 33), (16, 4, 64, 256, 40), (50, 3, 7, 65, 129),
-                 (129, 2, 1000, 64, 48), (400, 6, 24, 136, 200), (900, 2, 3, 72, 260), (700, 1, 1, 64, 520)]
+                 (129, 2, 1000, 64, 48), (400, 6, 24, 136, 200), (900, 2, 3, 72, 260), (700, 1, 1, 64, 520),
+                 (200, 2, 4, 72, 5000), (700, 2, 3, 72, 8200), (1100, 1, 1, 264, 12000), (700, 3, 9, 193, 2600)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -237,7 +267,8 @@ def test_expert_products_of_whole_numbers_are_exact(tokens, slots, experts, k, n
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("tokens,slots,experts,k,n", [(1, 8, 32, 1024, 96), (64, 4, 16, 520, 130), (600, 2, 6, 256, 192)])
+@pytest.mark.parametrize("tokens,slots,experts,k,n", [(1, 8, 32, 1024, 96), (2, 8, 32, 1030, 96), (64, 4, 16, 520, 130),
+                                                      (600, 2, 6, 256, 192), (600, 2, 4, 4200, 4160)])
 def test_expert_gate_up_and_combine_of_normal_values(tokens, slots, experts, k, n, dtype):
     torch, dense = _setup()
     dt = _dtype(torch, dtype)

@@ -70,13 +70,13 @@ def test_linear_refuses_a_short_workspace():
 
 
 def test_expert_linear_refuses_a_short_workspace():
-    p = _p()
+    p = _p(out_dim=4096)
     need = capi.lib().aeon_expert_linear_workspace_bytes(C.byref(p), 4, 9000)
     assert need > 0 and need % 16 == 0
     assert capi.lib().aeon_expert_linear_workspace_bytes(C.byref(p), 4, 8) == 0
     for ws, wb in ((None, need), (A, need - 1), (C.c_void_p((1 << 20) + 4), need)):
         with pytest.raises(ValueError, match="workspace of"):
-            _experts(p, x_rows=9000, positions=9000, ws=ws, wb=wb)
+            _experts(p, es=64 * 4096, x_rows=9000, positions=9000, ys=4096, ws=ws, wb=wb)
 
 
 @pytest.mark.parametrize("kw,text", [
