@@ -372,6 +372,46 @@ __device__ __forceinline__ void store_narrow(uint16_t* p, const float4_t& v, int
     }
 }
 
+// V (4 or 8) of a row's outputs in one 16-bit type, packed in pairs.
+template <class T, int V>
+struct Narrow {
+    typedef uint32_t packed_t __attribute__((ext_vector_type(V / 2)));
+    typedef packed_t __attribute__((aligned(2))) loose_t;
+    packed_t p;
+    __device__ __forceinline__ float value(int k) const { return T::widen(static_cast<uint16_t>(p[k / 2] >> (16 * (k & 1)))); }
+    __device__ __forceinline__ void round(const float (&v)[V]) {
+#pragma unroll
+        for (int k = 0; k < V; k += 2) p[k / 2] = T::round2(v[k], v[k + 1]);
+    }
+    __device__ __forceinline__ void load(const uint16_t* at, int o, int n) {
+        if (o + V <= n) {
+            p = *reinterpret_cast<const loose_t*>(at);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                if (k % 2 == 0) p[k / 2] = 0;
+                if (o + k < n) p[k / 2] |= static_cast<uint32_t>(at[k]) << (16 * (k & 1));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t* at, int o, int n) const {
+        if (o + V <= n) {
+            *reinterpret_cast<loose_t*>(at) = p;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (o + k < n) at[k] = static_cast<uint16_t>(p[k / 2] >> (16 * (k & 1)));
+        }
+    }
+};
+
+// Output of row r of a wave's ROWS panel rows of one matrix: in 32 rows the outputs of two 16-row tiles
+// are dealt out so that a lane's four rows of one tile and of the other follow each other.
+template <int ROWS>
+__device__ __forceinline__ int output_of(int r) {
+    return ROWS < 32 ? r : r / 32 * 32 + r % 16 / 4 * 8 + r % 32 / 16 * 4 + r % 4;
+}
+
 // The tile that fills a CU is run by waves that take turns (below).
 constexpr bool takes_turns(int bm, bool aligned) { return aligned && bm == 256; }
 
@@ -430,11 +470,13 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     for (int i = 0; i < NI; ++i) {
         const int r = panel_row(i) + (lane >> 3);
         if (r < BN) {
-            int matrix = 0, row = r;
-            if (a.pair) {
+            int matrix = 0, row;
+            if (a.pair) {  // a wave's first half are gate rows, its second half up rows
                 const int q = r % WN;
                 matrix = q >= WN / 2;
-                row = r / WN * (WN / 2) + q % (WN / 2);
+                row = r / WN * (WN / 2) + output_of<WN / 2>(q % (WN / 2));
+            } else {
+                row = r / WN * WN + output_of<WN>(r % WN);
             }
             row += n0;
             row = row < a.n ? row : a.n - 1;
@@ -671,102 +713,103 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
         multiply(f);
     }
 
-    // Epilogue. A lane holds outputs 4*(lane/16) .. +3 of a 16-row tile for position lane%16; the tile
-    // turns through LDS (the ring is done with, every wave has its own share) so that neighbouring
-    // lanes finish and store neighbouring outputs of one position: whole 128-byte lines, and one
-    // copy of the epilogue's code. The 16-byte units of a row are exclusive-ored with the row's
-    // number: neither side meets a bank twice.
-    constexpr int UNITS = WN / 4;  // of a position's row, gate and up together
-    constexpr int SHARE = S * STAGE / WAVES;
-    constexpr int CHUNK = WM * WN * 4 <= SHARE ? WM : WM / 2;  // positions turned at a time
-    static_assert(CHUNK * WN * 4 <= SHARE && CHUNK % 16 == 0 && UNITS <= 16, "the ring holds the turned tile");
-    wait_reads();
-    bare_barrier();
-    float4_t* turned = reinterpret_cast<float4_t*>(ring + wave * SHARE);
-    auto finish = [&](auto chunk, auto pair) __attribute__((always_inline)) {
-        constexpr int ROW = pair ? UNITS / 2 : UNITS;  // lanes of a position, four outputs each
-        constexpr int STEP = 64 / ROW;                 // positions a wave finishes at once
-        constexpr int EACH = CHUNK / STEP < 4 ? CHUNK / STEP : 4;  // of them in a row, to overlap their loads
-        const int turn_u = lane % ROW;
-        const int o = n0 + wave_n * (ROW * 4) + turn_u * 4;
-        const int from = position_of(wave_m * WM + chunk * CHUNK);
-        const int live = o < a.n ? t.count - from : 0;
-        const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        float4_t bias[2] = {zero, zero};  // the same for every position
-        if (a.mode != kProductPartial && o < a.n) {
-            const size_t at = static_cast<size_t>(t.expert) * a.n + o;
-            if (a.bias[0] != nullptr) bias[0] = load_narrow<T>(a.bias[0] + at, o, a.n);
-            if (pair && a.bias[1] != nullptr) bias[1] = load_narrow<T>(a.bias[1] + at, o, a.n);
+    // Epilogue. To the matrix instruction lane l is position l%16 and rows 4*(l/16) .. +3 of a 16-row
+    // tile. The panel's rows are not in the order of the outputs, though (output_of): two neighbouring
+    // tiles give a lane eight outputs in a row and a position's four lanes 32, 64 or 128 bytes, so results
+    // go to memory from where they are. (Turned through LDS into whole lines: 7.3 us a 256 x 256 tile.)
+    int to[TM];  // row of the output, or draw; -1: nowhere
+    float scale[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+        const int m = position_of(wave_m * WM + j * 16) + (lane & 15);
+        to[j] = m < t.count ? t.first + m : -1;
+        if (to[j] >= 0 && a.mode == kProductDraws) {
+            const int draw = a.draws[to[j]];
+            to[j] = draw >= 0 && draw < a.draw_count ? draw : -1;
+            scale[j] = to[j] >= 0 ? a.draw_weights[draw] : 0.0f;
+        } else if (to[j] >= 0 && a.rows != nullptr) {
+            const int row = a.rows[to[j]];
+            if (row < 0 || row >= a.x_rows) to[j] = -1;
         }
-#pragma unroll 1
-        for (int r0 = lane / ROW; r0 - lane / ROW < CHUNK; r0 += EACH * STEP) {
-            float4_t g[EACH], u[EACH], res[EACH];
-            float scale[EACH];
-            long draw[EACH];
-            bool ok[EACH];
+    }
+    auto finish = [&](auto pair) __attribute__((always_inline)) {
+        constexpr int TILES = pair ? TN / 2 : TN;   // of outputs
+        constexpr int RUN = TILES >= 2 ? 2 : 1;     // tiles that share a lane's outputs in a row
+        constexpr int V = RUN * 4, GROUPS = TILES / RUN;
+        const int o0 = n0 + wave_n * TILES * 16 + (lane >> 4) * V;  // outputs of group g: o0 + 32 g .. + V - 1
+        if (a.mode == kProductPartial) {
+            const size_t share = static_cast<size_t>(blockIdx.y) * (a.pair + 1) * a.positions;
 #pragma unroll
-            for (int k = 0; k < EACH; ++k) {
-                const int r = r0 + k * STEP, p = t.first + from + r;
-                g[k] = turned[r * UNITS + (turn_u ^ (r & (UNITS - 1)))];
-                u[k] = pair ? turned[r * UNITS + ((turn_u + UNITS / 2) ^ (r & (UNITS - 1)))] : zero;
-                ok[k] = r < live;
-                if (a.mode == kProductDraws && ok[k]) {
-                    draw[k] = a.draws[p];
-                    ok[k] = draw[k] >= 0 && draw[k] < a.draw_count;
-                    scale[k] = ok[k] ? a.draw_weights[draw[k]] : 0.0f;
-                }
-                if (a.rows != nullptr && ok[k]) ok[k] = a.rows[p] >= 0 && a.rows[p] < a.x_rows;
-                res[k] = zero;
-                if (a.residual != nullptr && ok[k])
-                    res[k] = load_narrow<T>(a.residual + p * a.residual_stride + o, o, a.n);
-            }
-            if (a.mode == kProductPartial) {
+            for (int j = 0; j < TM; ++j) {
+                if (to[j] < 0) continue;
 #pragma unroll
-                for (int k = 0; k < EACH; ++k) {
-                    if (!ok[k]) continue;
-                    const size_t p = t.first + from + r0 + k * STEP;
-                    float* dst = a.wide + (static_cast<size_t>(blockIdx.y) * (a.pair + 1) * a.positions + p) * a.n + o;
-                    store_wide(dst, g[k], o, a.n);
-                    if (pair) store_wide(dst + static_cast<size_t>(a.positions) * a.n, u[k], o, a.n);
-                }
-            } else if (a.mode == kProductDraws) {
-#pragma unroll
-                for (int k = 0; k < EACH; ++k)
-                    if (ok[k]) store_wide(a.wide + static_cast<size_t>(draw[k]) * a.n + o, (g[k] + bias[0]) * scale[k], o, a.n);
-            } else {
-                float y[EACH * 4], up[EACH * 4];
-#pragma unroll
-                for (int k = 0; k < EACH * 4; ++k) {
-                    y[k] = g[k / 4][k % 4] + bias[0][k % 4];
-                    up[k] = u[k / 4][k % 4] + bias[1][k % 4];
-                }
-                activate(a.activation, y, up, a.limit);
-#pragma unroll
-                for (int k = 0; k < EACH; ++k) {
-                    if (!ok[k]) continue;
-                    const int p = t.first + from + r0 + k * STEP;
-                    store_narrow<T>(a.y + p * a.y_stride + o,
-                                    float4_t{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]} + res[k], o, a.n);
+                for (int i = 0; i < TN; ++i) {
+                    const int o = o0 + i % TILES / RUN * 32 + i % RUN * 4;
+                    store_wide(a.wide + (share + static_cast<size_t>(i / TILES) * a.positions + to[j]) * a.n + o, acc[i][j], o, a.n);
                 }
             }
+            return;
+        }
+        float4_t bias[TN];  // the same for every position
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const int o = o0 + i % TILES / RUN * 32 + i % RUN * 4;
+            const uint16_t* from = a.bias[i / TILES];
+            bias[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (from != nullptr && o < a.n) bias[i] = load_narrow<T>(from + static_cast<size_t>(t.expert) * a.n + o, o, a.n);
+        }
+        if (a.mode == kProductDraws) {
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                if (to[j] < 0) continue;
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const int o = o0 + i / RUN * 32 + i % RUN * 4;
+                    store_wide(a.wide + static_cast<size_t>(to[j]) * a.n + o, (acc[i][j] + bias[i]) * scale[j], o, a.n);
+                }
+            }
+            return;
+        }
+        Narrow<T, V> ahead[GROUPS];  // residuals of the next position, asked for before this one's stores
+        auto residuals = [&](int row) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+                if (row >= 0) ahead[g].load(a.residual + row * a.residual_stride + o0 + 32 * g, o0 + 32 * g, a.n);
+        };
+        if (a.residual != nullptr) residuals(to[0]);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            Narrow<T, V> res[GROUPS];
+            if (a.residual != nullptr) {
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) res[g] = ahead[g];
+                if (j + 1 < TM) residuals(to[(j + 1) % TM]);
+            }
+            float y[TILES * 4], u[TILES * 4];
+#pragma unroll
+            for (int k = 0; k < TILES * 4; ++k) {
+                y[k] = acc[k / 4][j][k % 4] + bias[k / 4][k % 4];
+                u[k] = pair ? acc[(k / 4 + TILES) % TN][j][k % 4] + bias[(k / 4 + TILES) % TN][k % 4] : 0.0f;
+            }
+            activate(a.activation, y, u, a.limit);
+            if (to[j] < 0) continue;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                float v[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    v[k] = y[g * V + k];
+                    if (a.residual != nullptr) v[k] += res[g].value(k);
+                }
+                Narrow<T, V> out;
+                out.round(v);
+                out.store(a.y + to[j] * a.y_stride + o0 + 32 * g, o0 + 32 * g, a.n);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // one position at a time: the accumulators fill the registers
         }
     };
-    auto chunks = [&](auto chunk) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < CHUNK / 16; ++j) {
-            const int r = j * 16 + (lane & 15);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                turned[r * UNITS + ((i * 4 + (lane >> 4)) ^ (r & (UNITS - 1)))] = acc[i][chunk * (CHUNK / 16) + j];
-            }
-        }
-        asm volatile("" ::: "memory");  // LDS serves a wave's accesses in order
-        if (a.pair) finish(chunk, std::true_type{});
-        else finish(chunk, std::false_type{});
-        asm volatile("" ::: "memory");
-    };
-    chunks(C<0>{});
-    if constexpr (WM / CHUNK > 1) chunks(C<1>{});
+    if (a.pair) finish(std::true_type{});
+    else finish(std::false_type{});
 }
 
 // ---- a few positions: one pass of the weights through registers ------------------------------------
