@@ -421,8 +421,8 @@ const float* aeon_moe_layer_logits(const aeon_moe_layer* layer, int tokens, void
 /* One weight matrix (two for the gated activation), or one per expert, and what follows the
  * product. Every 16-bit operand of a call (activations, weights, biases, residual, output) is of
  * `dtype`; products and sums are fp32, and the result is rounded once. Any in_dim, out_dim and
- * pitch is taken; bases on 16-byte boundaries and pitches that are multiples of 8 elements run
- * the faster kernels. */
+ * pitch is taken; rows of activations and weights that all start on 4-byte boundaries (bases so
+ * aligned, even pitches) run the faster kernels. */
 typedef struct {
     int dtype;
     int in_dim;
@@ -453,13 +453,11 @@ int aeon_linear(const aeon_projection* projection, const void* d_x, long x_strid
  * expert_offsets[e+1]-1 are its list (aeon_expert_permutation), so that
  * y[p] = round(act(W_e x[row_indices[p]] + bias_e)); without row_indices row p itself. d_x has x_rows
  * rows. Rows of y behind the last list, and those of a position whose row index is outside
- * [0, x_rows), are left as they were. An expert without positions is not read. The workspace (16-byte
- * boundary) holds the tiles of long lists; short ones need none. */
-size_t aeon_expert_linear_workspace_bytes(const aeon_projection* projection, int experts, int positions);
+ * [0, x_rows), are left as they were. An expert without positions is not read. */
 int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,
                        const void* d_x, long x_stride, int x_rows, const int32_t* d_expert_offsets,
                        const int32_t* d_row_indices, int positions, void* d_y, long y_stride,
-                       void* d_workspace, size_t workspace_bytes, void* stream);
+                       void* stream);
 
 /* The down projection and the way back to tokens, the unquantised counterpart of
  * dispatch_aeon_moe_grouped_w2_wmma + the fixed-order reduce (moe_grouped_dispatch.hpp:66-88,
@@ -469,8 +467,7 @@ int aeon_expert_linear(const aeon_projection* projection, int experts, long expe
  * contributions stay fp32 (in the workspace, 16-byte boundary; a token or two need none). A slot whose id is outside
  * [0, experts) contributes nothing. d_base is nullable and may be d_out (same pitch). The projection
  * has no activation. d_h has tokens * slots rows, by position. */
-size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int experts, int tokens,
-                                           int slots);
+size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots);
 int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,
                         const void* d_h, long h_stride, const int32_t* d_expert_offsets,
                         const int32_t* d_draw_indices, const int32_t* d_topk_ids,

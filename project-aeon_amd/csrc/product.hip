@@ -156,22 +156,13 @@ __device__ __forceinline__ void patch_of(int u, int windows, int row_blocks, int
 
 // Tile of workgroup b. Workgroups are dealt to the 8 XCDs round robin, so tiles are handed out in 8
 // contiguous runs, one per XCD: neighbouring tiles share panels through one L2.
-// TURNS: one workgroup fills a CU, and a tile with at most half of its positions costs half. Where at
+// TURNS: one workgroup fills a CU, and a tile with at most half of its positions is cheaper. Where at
 // most half of the CUs would have a tile in an XCD's last round, a dense product's tiles of that round
-// are cut in two (the second part of a short one is empty); the tiles of lists come from a table.
+// are cut in two (the second part of a short one is empty).
 template <int BM, bool TURNS>
 __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, int b, ProductTile* t) {
-    if (TURNS && a.tiles != nullptr) {
-        const int4 entry = a.tiles[b];
-        t->expert = entry.x;
-        t->first = entry.y;
-        t->count = entry.z;
-        t->row_block = entry.w;
-        t->only = false;
-        return entry.z > 0;
-    }
     const int lane = threadIdx.x & 63;
-    const bool lists = !TURNS && a.offsets != nullptr;
+    const bool lists = a.offsets != nullptr;
     const int per = lists ? (a.experts + 63) / 64 : 0;  // experts a lane looks after
     int mine = 0, upto = 0, total;
     if (!lists) {
@@ -191,7 +182,7 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
     }
     const int run = (total + kXcds - 1) / kXcds;
     int at = b / kXcds, half = -1;
-    if (TURNS) {
+    if (TURNS && !lists) {
         const int last = run % kXcdCus;
         if (last <= kXcdCus / 2 && at >= run - last) {
             half = (at - (run - last)) & 1;
@@ -203,7 +194,9 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
     int expert = 0, first = 0, held = a.positions, before = 0;
     if (lists) {
         before = upto - mine;
-        const int from = __builtin_ctzll(__ballot(tile >= before * row_blocks && tile < upto * row_blocks));
+        const uint64_t owner = __ballot(tile >= before * row_blocks && tile < upto * row_blocks);
+        if (owner == 0) return false;  // only where the bounds do not ascend
+        const int from = __builtin_ctzll(owner);
         for (int e = lane * per; e < (lane + 1) * per && e < a.experts; ++e) {
             expert = e;
             held = list_of(a, e, &first);
@@ -229,81 +222,6 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
         if (half == 0 && t->count > BM / 2) t->count = BM / 2;
     }
     return t->count > 0;
-}
-
-// The tiles of lists for the kernel whose workgroups fill a CU, one entry a workgroup: {expert, first
-// position, positions (0: nothing to do), row block}. A list is its windows of more than half the
-// positions, then perhaps one shorter that costs half. The XCDs' runs are cut at equal cost: with the
-// popular experts first, equal numbers of tiles gave the first XCD a fifth more work than the mean.
-// One workgroup, a thread an expert, then the threads over the entries.
-__global__ __launch_bounds__(1024) void product_tiles_kernel(const ProductArgs a, int bm, int row_blocks, int entries,
-                                                             int4* table) {
-    __shared__ int cost_before[1025], tiles_before[1025], wave_cost[16], wave_tiles[16], run_from[kXcds + 1];
-    const int e = threadIdx.x, lane = e & 63, wave = e >> 6;
-    auto wholes_of = [&](int n) { return n / bm + (n % bm > bm / 2); };
-    auto windows_of = [&](int n) { return (n + bm - 1) / bm; };
-    int first, held = 0;
-    if (e < a.experts) held = list_of(a, e, &first);
-    int cost = wholes_of(held) + windows_of(held), tiles = windows_of(held);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int c = __shfl_up(cost, d, 64), n = __shfl_up(tiles, d, 64);
-        if (lane >= d) {
-            cost += c;
-            tiles += n;
-        }
-    }
-    if (lane == 63) {
-        wave_cost[wave] = cost;
-        wave_tiles[wave] = tiles;
-    }
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-        cost += wave_cost[w];
-        tiles += wave_tiles[w];
-    }
-    cost_before[e + 1] = cost;
-    tiles_before[e + 1] = tiles;
-    if (e == 0) cost_before[0] = tiles_before[0] = 0;
-    __syncthreads();
-    auto holder = [&](const int* before, int v) {  // the expert whose share of the prefix holds v
-        int lo = 0, hi = 1024;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (before[mid] * row_blocks <= v) lo = mid;
-            else hi = mid;
-        }
-        return lo;
-    };
-    if (e <= kXcds) {  // the first tile that starts at an eighth of the cost or later
-        const int all = cost_before[1024] * row_blocks;
-        const int c = static_cast<int>(static_cast<long>(all) * e / kXcds);
-        int tile = tiles_before[1024] * row_blocks;
-        if (c < all) {
-            const int x = holder(cost_before, c);
-            int dummy;
-            const int in = c - cost_before[x] * row_blocks;
-            const int whole_cost = 2 * wholes_of(list_of(a, x, &dummy)) * row_blocks;
-            tile = tiles_before[x] * row_blocks + (in <= whole_cost ? (in + 1) / 2 : whole_cost / 2 + in - whole_cost);
-        }
-        run_from[e] = tile;
-    }
-    __syncthreads();
-    for (int b = threadIdx.x; b < entries; b += 1024) {
-        const int tile = run_from[b % kXcds] + b / kXcds;
-        int4 entry = make_int4(0, 0, 0, 0);
-        if (tile < run_from[b % kXcds + 1]) {
-            const int x = holder(tiles_before, tile);
-            int from;
-            const int n = list_of(a, x, &from), wholes = wholes_of(n);
-            const int u = tile - tiles_before[x] * row_blocks;
-            int window = wholes, block = u - wholes * row_blocks;
-            if (block < 0) patch_of(u, wholes, row_blocks, &window, &block);
-            const int rest = n - window * bm;
-            entry = make_int4(x, from + window * bm, rest < bm ? rest : bm, block);
-        }
-        table[b] = entry;
-    }
 }
 
 // 16 bytes of a row starting at column c, zeros from column k on. `p` is the row's column 0; nothing
@@ -1090,38 +1008,36 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, 
 }
 
 // out[t][i] = round(base[t][i] + sum of the token's contributions in slot order). A draw whose id
-// is outside [0, experts) holds no contribution and is left out.
+// is outside [0, experts) holds no contribution and is left out. Four outputs a thread, one token a
+// workgroup, eight slots' loads in flight.
 template <class T>
 __global__ __launch_bounds__(256) void product_combine_kernel(const float* __restrict__ contrib,
                                                               const int32_t* __restrict__ ids, int experts,
-                                                              int tokens, int slots, int n, const uint16_t* base,
+                                                              int blocks, int slots, int n, const uint16_t* base,
                                                               long base_stride, uint16_t* out, long out_stride) {
-    const int groups = (n + 3) / 4;
-    const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= static_cast<long>(tokens) * groups) return;
-    const int t = static_cast<int>(at / groups);
-    const int o = static_cast<int>(at - static_cast<long>(t) * groups) * 4;
-    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (base != nullptr) v = load_narrow<T>(base + t * base_stride + o, o, n);
-    for (int s = 0; s < slots; ++s) {
-        const long draw = static_cast<long>(t) * slots + s;
-        const int id = ids[draw];
-        if (id >= 0 && id < experts) v += load_wide(contrib + static_cast<size_t>(draw) * n + o, o, n);
+    const int t = blockIdx.x / blocks;
+    const int o = ((blockIdx.x - t * blocks) * 256 + threadIdx.x) * 4;
+    if (o >= n) return;
+    const long draw = static_cast<long>(t) * slots;
+    float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (base != nullptr) sum = load_narrow<T>(base + t * base_stride + o, o, n);
+    for (int s = 0; s < slots; s += 8) {
+        float4_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int id = s + k < slots ? ids[draw + s + k] : -1;
+            v[k] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (id >= 0 && id < experts) v[k] = load_wide(contrib + static_cast<size_t>(draw + s + k) * n + o, o, n);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += v[k];
     }
-    store_narrow<T>(out + t * out_stride + o, v, o, n);
+    store_narrow<T>(out + t * out_stride + o, sum, o, n);
 }
 
 // ---- launches --------------------------------------------------------------------------------
 
-constexpr int kTurnsTile = 256;
-
-// Entries of the tile table: an XCD's run is an eighth of the cost, which is that many tiles if every
-// one of them costs half.
-static long table_entries(int n, bool pair, int experts, int positions) {
-    const long row_blocks = (n * (pair ? 2L : 1L) + kTurnsTile - 1) / kTurnsTile;
-    const long lists = experts < positions ? experts : positions;
-    return ((positions / (kTurnsTile / 2) + lists) * row_blocks / kXcds + 2) * kXcds;
-}
+constexpr int kLargestTile = 256;
 
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N, int S, bool ALIGNED>
 static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
@@ -1145,18 +1061,10 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
     long windows = (static_cast<long>(a.positions) + BM - 1) / BM;
     if (a.offsets != nullptr) windows = a.positions / BM + (a.experts < a.positions ? a.experts : a.positions);
     long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
-    if (BM == kTurnsTile && ALIGNED) {
-        if (a.offsets == nullptr) grid += kXcds * (kXcdCus / 2);  // room for a last round in halves
-        else grid = table_entries(a.n, a.pair, a.experts, a.positions);
-    }
+    // room for a last round in halves
+    if (takes_turns(BM, ALIGNED) && a.offsets == nullptr) grid += kXcds * (kXcdCus / 2);
     AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
-    ProductArgs args = a;
-    if (BM == kTurnsTile && ALIGNED && a.offsets != nullptr) {
-        product_tiles_kernel<<<1, 1024, 0, stream>>>(a, BM, static_cast<int>(row_blocks), static_cast<int>(grid), a.table);
-        AEON_LAUNCH_CHECK();
-        args.tiles = a.table;
-    }
-    kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(args);
+    kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(a);
     AEON_LAUNCH_CHECK();
     return AEON_OK;
 }
@@ -1229,7 +1137,7 @@ struct TileCost {
     double step_alone, step_shared, fixed;
 };
 constexpr TileCost kTileCosts[] = {{16, 64, 0.12, 0.27, 2.8}, {32, 64, 0.16, 0.34, 3.0}, {64, 64, 0.21, 0.40, 2.9},
-                                   {128, 128, 0.68, 1.04, 4.1}, {kTurnsTile, kTurnsTile, 1.38, 0.0, 18.8}};
+                                   {128, 128, 0.68, 1.04, 4.1}, {kLargestTile, kLargestTile, 1.38, 0.0, 18.8}};
 
 // Every tile and number of shares priced: rounds of workgroups, the weights' way from memory, and the
 // second launch that joins shares with its traffic.
@@ -1249,7 +1157,7 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
             const int each = (steps + splits - 1) / splits;
             const long groups = static_cast<long>(tiles * splits);
             double us;
-            if (t.positions == kTurnsTile) {
+            if (t.positions == kLargestTile) {
                 const long last = groups % 256;
                 const double half = 0.55;  // of a tile's products, where its positions or its last round fill one half
                 us = groups / 256 * (each * t.step_alone + t.fixed);
@@ -1283,7 +1191,7 @@ static int plan_experts(const aeon_projection& w, int positions, int experts) {
     const int mean = positions / (live > 0 ? live : 1);
     const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
-    if (mean > 112 && tiles(256) >= 192) return kTurnsTile;
+    if (mean > 112 && tiles(256) >= 192) return kLargestTile;
     if (mean > 48 && tiles(128) >= 192) return 128;
     return mean <= 12 ? 16 : mean <= 24 ? 32 : 64;
 }
@@ -1337,17 +1245,6 @@ static int check_experts(const aeon_projection& w, int experts, long expert_stri
 
 static bool combine_direct(const aeon_projection& w, int tokens, int slots) {
     return tokens <= kDirectTokens && static_cast<long>(tokens) * slots <= kDirectDraws && w.in_dim >= kFewColumns;
-}
-
-// Bytes of the tile table a product over lists needs.
-static size_t table_bytes(const aeon_projection& w, int experts, int positions) {
-    if (positions <= 0 || experts <= 0 || plan_experts(w, positions, experts) != kTurnsTile) return 0;
-    return static_cast<size_t>(table_entries(w.out_dim, w.activation == AEON_ACT_SWIGLU, experts, positions)) * sizeof(int4);
-}
-
-static size_t contrib_bytes(const aeon_projection& w, int tokens, int slots) {
-    const size_t bytes = static_cast<size_t>(tokens) * slots * w.out_dim * sizeof(float);
-    return (bytes + 15) / 16 * 16;
 }
 
 static int check_workspace(const void* d_workspace, size_t bytes, size_t need, const char* who) {
@@ -1414,15 +1311,10 @@ extern "C" int aeon_linear(const aeon_projection* projection, const void* d_x, l
     return AEON_OK;
 }
 
-extern "C" size_t aeon_expert_linear_workspace_bytes(const aeon_projection* projection, int experts, int positions) {
-    if (check_projection(projection, "aeon_expert_linear_workspace_bytes") != AEON_OK) return 0;
-    return table_bytes(*projection, experts, positions);
-}
-
 extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,
                                   const void* d_x, long x_stride, int x_rows, const int32_t* d_expert_offsets,
                                   const int32_t* d_row_indices, int positions, void* d_y, long y_stride,
-                                  void* d_workspace, size_t workspace_bytes, void* stream) {
+                                  void* stream) {
     const char* who = "aeon_expert_linear";
     if (int rc = check_projection(projection, who)) return rc;
     const aeon_projection& w = *projection;
@@ -1437,9 +1329,7 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
                  who, x_stride, y_stride);
     AEON_REQUIRE(d_y != d_x && d_y != w.d_weight && d_y != w.d_weight_up, AEON_ERR_INVALID_ARGUMENT,
                  "%s: the output must not alias the activations or the weights", who);
-    if (int rc = check_workspace(d_workspace, workspace_bytes, table_bytes(w, experts, positions), who)) return rc;
     ProductArgs a = projection_args(w);
-    a.table = static_cast<int4*>(d_workspace);
     a.expert_stride = expert_stride;
     a.x = static_cast<const uint16_t*>(d_x);
     a.x_stride = x_stride;
@@ -1453,11 +1343,11 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
     return launch_product(w.dtype, plan_experts(w, positions, experts), a, 1, as_stream(stream));
 }
 
-extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int experts, int tokens, int slots) {
+extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots) {
     if (check_projection(projection, "aeon_expert_combine_workspace_bytes") != AEON_OK || tokens <= 0 || slots <= 0 ||
         static_cast<long>(tokens) * slots > 0x7fffffffL || combine_direct(*projection, tokens, slots))
         return 0;
-    return contrib_bytes(*projection, tokens, slots) + table_bytes(*projection, experts, tokens * slots);
+    return static_cast<size_t>(tokens) * slots * projection->out_dim * sizeof(float);
 }
 
 extern "C" int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,
@@ -1485,7 +1375,7 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
                  "%s: the output must not alias the hidden rows or the weights", who);
     AEON_REQUIRE(d_out != d_base || out_stride == base_stride, AEON_ERR_INVALID_ARGUMENT,
                  "%s: an output on the base needs the base's row pitch", who);
-    const size_t need = aeon_expert_combine_workspace_bytes(projection, experts, tokens, slots);
+    const size_t need = aeon_expert_combine_workspace_bytes(projection, tokens, slots);
     if (int rc = check_workspace(d_workspace, workspace_bytes, need, who)) return rc;
     ProductArgs a = projection_args(w);
     a.expert_stride = expert_stride;
@@ -1497,7 +1387,6 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
     a.positions = tokens * slots;
     a.mode = kProductDraws;
     a.wide = static_cast<float*>(d_workspace);
-    a.table = reinterpret_cast<int4*>(static_cast<char*>(d_workspace) + contrib_bytes(w, tokens, slots));
     a.draws = d_draw_indices;
     a.draw_weights = d_topk_weights;
     a.draw_count = tokens * slots;
@@ -1513,15 +1402,16 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
         return AEON_OK;
     }
     if (int rc = launch_product(w.dtype, plan_experts(w, a.positions, experts), a, 1, as_stream(stream))) return rc;
-    const long threads = static_cast<long>(tokens) * ((w.out_dim + 3) / 4);
-    AEON_REQUIRE((threads + 255) / 256 <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "%s: too many outputs for one launch", who);
-    const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+    const int row_blocks = (w.out_dim + 1023) / 1024;
+    const long blocks = static_cast<long>(tokens) * row_blocks;
+    AEON_REQUIRE(blocks <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "%s: too many outputs for one launch", who);
+    const auto grid = static_cast<unsigned>(blocks);
     if (w.dtype == AEON_DTYPE_F16) {
-        product_combine_kernel<F16><<<blocks, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, tokens, slots, w.out_dim,
-                                                                          base, base_stride, out, out_stride);
+        product_combine_kernel<F16><<<grid, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, row_blocks, slots, w.out_dim,
+                                                                        base, base_stride, out, out_stride);
     } else {
-        product_combine_kernel<BF16><<<blocks, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, tokens, slots, w.out_dim,
-                                                                           base, base_stride, out, out_stride);
+        product_combine_kernel<BF16><<<grid, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, row_blocks, slots, w.out_dim,
+                                                                         base, base_stride, out, out_stride);
     }
     AEON_LAUNCH_CHECK();
     return AEON_OK;

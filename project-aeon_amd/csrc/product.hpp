@@ -37,8 +37,6 @@ struct ProductArgs {
     const int32_t* draws;      // kProductDraws: draw of a position
     const float* draw_weights; // by draw
     int draw_count;
-    int4* table;               // room for the tile table of lists, and
-    const int4* tiles;         // that table where the kernel reads one
     int split_steps;           // kProductPartial: 64-column steps of one share of K
 };
 

@@ -160,11 +160,8 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
     positions = x_rows if rows is None else rows.shape[0]
     _lists(device, weight.shape[0], offsets, positions, rows, "rows")
     out = _output(out, x, (positions, p.out_dim))
-    at, experts = C.addressof(p), weight.shape[0]
-    need = capi.lib().aeon_expert_linear_workspace_bytes(at, experts, positions)
-    ws = _workspace(x, need)
-    _call(device, "aeon_expert_linear", at, experts, _expert_stride(weight, p), x.data_ptr(), _pitch(x), x_rows,
-          offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), _pitch(out), _ptr(ws), need)
+    _call(device, "aeon_expert_linear", C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), _pitch(x),
+          x_rows, offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), _pitch(out))
     return out
 
 
@@ -189,7 +186,7 @@ def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None
         _check(base, "base", device, h.dtype, shape)
     out = _output(out, h, shape)
     at = C.addressof(p)
-    need = capi.lib().aeon_expert_combine_workspace_bytes(at, weight.shape[0], tokens, slots)
+    need = capi.lib().aeon_expert_combine_workspace_bytes(at, tokens, slots)
     ws = _workspace(h, need)
     _call(device, "aeon_expert_combine", at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), _pitch(h),
           offsets.data_ptr(), draws.data_ptr(), ids.data_ptr(), weights.data_ptr(), tokens, slots, _ptr(base),

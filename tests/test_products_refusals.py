@@ -22,9 +22,9 @@ def _linear(p, x=A, xs=64, tokens=4, res=None, rs=0, y=B, ys=32, ws=None, wb=0):
               ws, C.c_size_t(wb), None)
 
 
-def _experts(p, experts=4, es=2048, x=A, xs=64, x_rows=8, off=A, rows=None, positions=8, y=B, ys=32, ws=None, wb=0):
+def _experts(p, experts=4, es=2048, x=A, xs=64, x_rows=8, off=A, rows=None, positions=8, y=B, ys=32):
     capi.call("aeon_expert_linear", C.byref(p), experts, C.c_long(es), x, C.c_long(xs), x_rows, off, rows, positions, y,
-              C.c_long(ys), ws, C.c_size_t(wb), None)
+              C.c_long(ys), None)
 
 
 def _combine(p, experts=4, es=2048, h=A, hs=64, off=A, draws=A, ids=A, w=A, tokens=4, slots=2, base=None, bs=0, out=B,
@@ -47,7 +47,7 @@ def test_projection_refusals(change, text):
         with pytest.raises(ValueError, match=text):
             call(_p(**change))
     assert capi.lib().aeon_linear_workspace_bytes(C.byref(_p(**change)), 4) == 0
-    assert capi.lib().aeon_expert_combine_workspace_bytes(C.byref(_p(**change)), 4, 4, 2) == 0
+    assert capi.lib().aeon_expert_combine_workspace_bytes(C.byref(_p(**change)), 4, 2) == 0
 
 
 @pytest.mark.parametrize("kw,text", [
@@ -67,16 +67,6 @@ def test_linear_refuses_a_short_workspace():
     for ws, wb in ((None, need), (A, need - 1), (C.c_void_p((1 << 20) + 4), need)):
         with pytest.raises(ValueError, match="workspace of"):
             _linear(p, xs=7168, ys=256, tokens=20, ws=ws, wb=wb)
-
-
-def test_expert_linear_refuses_a_short_workspace():
-    p = _p(out_dim=4096)
-    need = capi.lib().aeon_expert_linear_workspace_bytes(C.byref(p), 4, 9000)
-    assert need > 0 and need % 16 == 0
-    assert capi.lib().aeon_expert_linear_workspace_bytes(C.byref(p), 4, 8) == 0
-    for ws, wb in ((None, need), (A, need - 1), (C.c_void_p((1 << 20) + 4), need)):
-        with pytest.raises(ValueError, match="workspace of"):
-            _experts(p, es=64 * 4096, x_rows=9000, positions=9000, ys=4096, ws=ws, wb=wb)
 
 
 @pytest.mark.parametrize("kw,text", [
