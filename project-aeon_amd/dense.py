@@ -33,16 +33,22 @@ class Projection(C.Structure):
 # reads, and one call costs the host about as much as one of torch's own element-wise operators.
 
 
+def _fits(t, device, dtype, shape):
+    """Of this type, on this GPU, of this shape, the elements of a row next to each other."""
+    return (t.dtype is dtype and t.get_device() == device and t.shape == shape
+            and (t.stride(-1) == 1 or t.shape[-1] <= 1))
+
+
 def _check(t, name, device, dtype, shape):
-    """One operand: of this type, on this GPU, of this shape, the elements of a row next to each other."""
+    if _fits(t, device, dtype, shape):
+        return
     if t.dtype is not dtype:
         raise ValueError("%s is %s, not %s" % (name, t.dtype, dtype))
     if t.get_device() != device:
         raise ValueError("%s is on %s, not on GPU %d" % (name, t.device, device))
     if t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError("%s: elements of a row have to follow each other" % name)
+    raise ValueError("%s: elements of a row have to follow each other" % name)
 
 
 def _pitch(t):
@@ -57,32 +63,35 @@ def _ptr(t):
 
 
 def _projection(x, weight, bias, activation, weight_up, bias_up, limit, lead):
-    dtype = _DTYPES.get(x.dtype)
-    if dtype is None or x.dim() != 2 or not x.is_cuda:
+    kind, shape, device = x.dtype, weight.shape, x.get_device()
+    dtype, act = _DTYPES.get(kind), ACTIVATIONS.get(activation)
+    if dtype is None or device < 0 or x.dim() != 2:
         raise ValueError("x has to be a 2-d fp16 or bf16 tensor on a GPU")
-    act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError("unknown activation %r" % (activation,))
-    shape = weight.shape
     if len(shape) != 2 + lead:
         raise ValueError("weight has to have %d dimensions" % (2 + lead))
     out_dim, in_dim = shape[-2], shape[-1]
-    device = x.get_device()
-    _check(x, "x", device, x.dtype, (x.shape[0], in_dim))
-    _check(weight, "weight", device, x.dtype, shape)
+    _check(x, "x", device, kind, (x.shape[0], in_dim))
+    _check(weight, "weight", device, kind, shape)
     stride = weight.stride(-2)
     if out_dim == 1 and stride < in_dim:
         stride = in_dim
     if weight_up is not None:
-        _check(weight_up, "weight_up", device, x.dtype, shape)
+        _check(weight_up, "weight_up", device, kind, shape)
         if weight_up.stride() != weight.stride():
             raise ValueError("weight and weight_up have to have the same strides")
-    for b, name in ((bias, "bias"), (bias_up, "bias_up")):
-        if b is not None:
-            _check(b, name, device, x.dtype, shape[:-1])
-            if not b.is_contiguous():
-                raise ValueError("%s has to be contiguous" % name)
+    if bias is not None:
+        _check_bias(bias, "bias", device, kind, shape)
+    if bias_up is not None:
+        _check_bias(bias_up, "bias_up", device, kind, shape)
     return Projection(dtype, in_dim, out_dim, act, weight.data_ptr(), _ptr(weight_up), stride, _ptr(bias), _ptr(bias_up), limit)
+
+
+def _check_bias(b, name, device, kind, shape):
+    _check(b, name, device, kind, shape[:-1])
+    if not b.is_contiguous():
+        raise ValueError("%s has to be contiguous" % name)
 
 
 def _call(device, name, *args):
