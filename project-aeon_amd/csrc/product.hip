@@ -7,15 +7,23 @@
 //
 // One workgroup computes BN weight rows x BM positions. Both panels of a 64-column step (rows of
 // 128 bytes) go from memory straight to LDS (16 bytes a lane, no registers) into a ring of S
-// stages; the requests for step s+S-1 are issued behind the barrier that opens step s, so S-1
-// steps are in flight while one is multiplied. A request instruction fills 8 rows; lane l writes
-// LDS unit l of them, and fetches unit (l%8) ^ (l/8) of row l/8: the exclusive-or spreads the
-// 16-byte units of 8 consecutive rows over all banks, so that the fragment reads (16 rows, one
-// unit each) are free of conflicts, while 8 neighbouring lanes still read 128 contiguous bytes.
+// stages. A request instruction fills 8 rows; lane l writes LDS unit l of them, and fetches unit
+// (l%8) ^ (l/8) of row l/8: the exclusive-or spreads the 16-byte units of 8 consecutive rows over
+// all banks, so that the fragment reads (16 rows, one unit each) are free of conflicts, while 8
+// neighbouring lanes still read 128 contiguous bytes.
 //
-// Weights are the A operand of v_mfma_f32_16x16x32: lane l ends with four consecutive outputs of
-// position l%16. The gated form keeps a wave's gate rows and up rows side by side in the panel,
+// Weights are the A operand of v_mfma_f32_16x16x32: a lane ends with four rows of each 16-row tile
+// for position l%16. The gated form keeps a wave's gate rows and up rows side by side in the panel,
 // so both pre-activations of an output meet in one lane.
+//
+// What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
+//   4 x any    the weight stream, by registers and VALU: 6.3 TB/s over the eight experts of one token
+//   16..64     the weight stream while it is long: 7.0 TB/s over 12.9 GB (64 tokens, 256 experts); in
+//              short products a workgroup's own start and end, and with 64 positions LDS and the way
+//              from L2 to it (about 80 GB/s a CU)
+//   128, 256   the matrix pipe: a 256 x 256 x 64 step takes 1.36 us where the panels are in L2, 1.58
+//              PFLOP/s; 2.07 us where every weight panel is one workgroup's own and comes from
+//              HBM, because a CU's 64 KB a step then wait for misses of twice the latency
 #include "product.hpp"
 
 #include <atomic>
@@ -467,14 +475,17 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
     };
 
     if constexpr (TURNS) {
-        // Two waves share a SIMD; they take turns at its matrix pipe. A step is four quarters of
-        // the wave's tile, and a quarter a fetch part (LDS reads, requests) and a multiply part,
-        // each ended by a barrier; waves 4..7 run one barrier behind waves 0..3, so that one wave
-        // of a SIMD fetches while the other multiplies. A part's LDS reads have landed when its
-        // barrier opens, so the region they came from is asked for again, for two steps later, one
-        // fetch part on; a part waits for what the next one reads, by the number of the wave's
-        // younger requests. Up to 14 are under way per wave, 112 KB of a CU's 128 KB of panels.
-        // (A third stage of weights in the 32 KB that are left: 2 % slower.)
+        // Two waves share a SIMD; they take turns at its matrix pipe. A step is two parts of 32
+        // MFMAs a wave, one for each half of its positions, and a part a fetch (LDS reads, requests)
+        // and a multiply, each ended by a barrier; waves 4..7 run one barrier behind waves 0..3, so
+        // that one wave of a SIMD fetches while the other multiplies. A fetch's LDS reads have landed
+        // when its barrier opens, so the region they came from is asked for again, for the next use of
+        // its stage, in the fetch after that; a fetch waits for what the next one reads, by the number
+        // of the wave's younger requests. Up to 14 are under way per wave, 112 KB of the 128 KB of
+        // panels. Measured at 8192 x 8192, K 7168: both waves in step 1017 us, turns of 16 MFMAs 727,
+        // of 32 664. A third stage of weights in the LDS that is left: 2 % slower. Workgroups that
+        // stay and ask for the next tile's first panels before they store: no faster (61 us against
+        // 58 for four tiles of one step), as requests wait behind stores.
         u32x4_t wf[2][2][2], xf[4][2];  // [half of the weight rows][tile][columns 32h..], [tile][columns]
         auto read_w = [&](int stage, auto half) __attribute__((always_inline)) {
             const char* wp = ring + stage * STAGE + (wave_n * WN + half * (WN / 2)) * kStepBytes;
@@ -541,7 +552,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N) void product_kernel(const P
                 part(C<1>{}, C<1>{}, C<1>{});
             }
         } else {
-            // no second half of positions: two quarters and six requests a step
+            // no second half of positions: parts of 16 MFMAs, one for each half of the weight rows, and
+            // six requests a step, which make it 0.75 of a whole one
             if (full > 0) request(0, 0, C<0>{}, C<6>{}, kept);
             if (full > 1) {
                 request(1, 1, C<0>{}, C<4>{}, kept);
@@ -1070,7 +1082,7 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
 }
 
 // Rows of each matrix a workgroup of the few-position kernel takes: eight loads in flight a wave, or
-// fewer where that would leave CUs without a workgroup.
+// fewer where that would leave CUs without a workgroup (2 a CU at least).
 template <class T, int ROWS, int MATS>
 static int launch_few_rows(const ProductArgs& a, long windows, hipStream_t stream) {
     const long grid = (windows * ((a.n + ROWS - 1) / ROWS) + kXcds - 1) / kXcds * kXcds;
@@ -1122,16 +1134,18 @@ static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipSt
     return aligned ? launch_tiles<BF16, true>(tile, a, splits, stream) : launch_tiles<BF16, false>(tile, a, splits, stream);
 }
 
+constexpr int kMostPositions = 1 << 30;  // positions and their sums with a tile's are 32-bit numbers
+
 // Positions a tile holds and the shares K is cut into.
 struct ProductPlan {
     int tile, splits, split_steps;
 };
 
 // What a tile costs, us: a 64-column step of a workgroup that has its CU to itself, of one of two that
-// share it, and the rest of a workgroup (launch, first requests, epilogue). Least squares over products of
+// share it, and the rest of a workgroup (launch, first requests, epilogue). Fitted to products of
 // 5 to 4096 tokens with matrices of 512 x 1024 to 7168 x 7168, each at every tile and at one to eight
-// shares, weights cold (72 products; the plan made from these figures is within 0.9 % of the best one
-// measured in the mean, and 16 % at worst).
+// shares, weights cold (72 products; the plan made from these figures is within 1.2 % of the best one
+// measured in the mean, and 18 % at worst).
 struct TileCost {
     int positions, rows;
     double step_alone, step_shared, fixed;
@@ -1182,17 +1196,19 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
 
 // Lists: by how many positions an expert holds on average, and only as large a tile as leaves the CUs
 // enough of them (half a window an expert is taken to be short). Measured, us per product at a mean of 16 /
-// 32 / 64 / 96 / 128 / 192 positions, 64 experts of 4096 x 2048: tile 32: 172 / 222 / 317; 64: 168 / 193 /
-// 259 / 312 / 385; 128: 188 / 206 / 229 / 262 / 303 / 384; 256: 221 / 223 / 232 / 274 / 286 / 278. Eight experts of 4096 x 4096
-// at 192: tile 64 118, 128 77, 256 93; at 256: 151, 135, 99.
+// 32 / 64 / 96 / 128 / 192 positions, 64 experts of 4096 x 2048: tile 32: 172 / 222 / 316 / 407 / 498 / 689;
+// 64: 168 / 189 / 262 / 306 / 361 / 489; 128: 185 / 202 / 221 / 240 / 288 / 356; 256: 204 / 207 / 214 / 219 /
+// 234 / 273. Gated, 2048 outputs of 4096 columns, at 64 / 96 / 128: 128: 385 / 403 / 528, 256: 408 / 405 /
+// 428. Eight experts of 4096 x 4096, tile 64 / 128 / 256, at 96: 66 / 72 / 66; at 192: 106 / 76 / 87; at 256:
+// 146 / 131 / 92.
 static int plan_experts(const aeon_projection& w, int positions, int experts) {
     if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kFewMax;
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
     const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
-    if (mean > 112 && tiles(256) >= 192) return kLargestTile;
-    if (mean > 48 && tiles(128) >= 192) return 128;
+    if (mean > 80 && tiles(kLargestTile) >= 192) return kLargestTile;
+    if (mean > 48 && tiles(128) >= 400) return 128;
     return mean <= 12 ? 16 : mean <= 24 ? 32 : 64;
 }
 
@@ -1237,7 +1253,8 @@ static ProductArgs projection_args(const aeon_projection& w) {
 
 static int check_experts(const aeon_projection& w, int experts, long expert_stride, int positions, const char* who) {
     AEON_REQUIRE(experts > 0 && experts <= 1024, AEON_ERR_INVALID_ARGUMENT, "%s: expert count out of range (%d)", who, experts);
-    AEON_REQUIRE(positions >= 0, AEON_ERR_INVALID_ARGUMENT, "%s: negative count", who);
+    AEON_REQUIRE(positions >= 0 && positions <= kMostPositions, AEON_ERR_INVALID_ARGUMENT, "%s: position count out of range (%d)",
+                 who, positions);
     AEON_REQUIRE(expert_stride >= (w.out_dim - 1) * w.weight_stride + w.in_dim, AEON_ERR_INVALID_ARGUMENT,
                  "%s: expert matrices %ld elements apart overlap", who, expert_stride);
     return AEON_OK;
@@ -1264,7 +1281,7 @@ static size_t linear_workspace(const aeon_projection& w, int tokens, const Produ
 using namespace aeon355;
 
 extern "C" size_t aeon_linear_workspace_bytes(const aeon_projection* projection, int tokens) {
-    if (check_projection(projection, "aeon_linear_workspace_bytes") != AEON_OK || tokens <= 0) return 0;
+    if (check_projection(projection, "aeon_linear_workspace_bytes") != AEON_OK || tokens <= 0 || tokens > kMostPositions) return 0;
     return linear_workspace(*projection, tokens, plan_linear(*projection, tokens));
 }
 
@@ -1274,7 +1291,7 @@ extern "C" int aeon_linear(const aeon_projection* projection, const void* d_x, l
     const char* who = "aeon_linear";
     if (int rc = check_projection(projection, who)) return rc;
     const aeon_projection& w = *projection;
-    AEON_REQUIRE(tokens >= 0, AEON_ERR_INVALID_ARGUMENT, "%s: negative token count", who);
+    AEON_REQUIRE(tokens >= 0 && tokens <= kMostPositions, AEON_ERR_INVALID_ARGUMENT, "%s: token count out of range (%d)", who, tokens);
     if (tokens == 0) return AEON_OK;
     AEON_REQUIRE(d_x && d_y, AEON_ERR_INVALID_ARGUMENT, "%s: null buffer", who);
     AEON_REQUIRE(on_boundary(d_x, 2) && on_boundary(d_y, 2) && on_boundary(d_residual, 2), AEON_ERR_INVALID_ARGUMENT,
@@ -1345,7 +1362,7 @@ extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts
 
 extern "C" size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots) {
     if (check_projection(projection, "aeon_expert_combine_workspace_bytes") != AEON_OK || tokens <= 0 || slots <= 0 ||
-        static_cast<long>(tokens) * slots > 0x7fffffffL || combine_direct(*projection, tokens, slots))
+        static_cast<long>(tokens) * slots > kMostPositions || combine_direct(*projection, tokens, slots))
         return 0;
     return static_cast<size_t>(tokens) * slots * projection->out_dim * sizeof(float);
 }
@@ -1360,7 +1377,7 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
     if (int rc = check_projection(projection, who)) return rc;
     const aeon_projection& w = *projection;
     AEON_REQUIRE(w.activation == AEON_ACT_NONE, AEON_ERR_INVALID_ARGUMENT, "%s: takes no activation", who);
-    AEON_REQUIRE(tokens >= 0 && slots > 0 && static_cast<long>(tokens) * slots <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT,
+    AEON_REQUIRE(tokens >= 0 && slots > 0 && static_cast<long>(tokens) * slots <= kMostPositions, AEON_ERR_INVALID_ARGUMENT,
                  "%s: bad draw shape (tokens=%d slots=%d)", who, tokens, slots);
     if (int rc = check_experts(w, experts, expert_stride, tokens * slots, who)) return rc;
     if (tokens == 0) return AEON_OK;

@@ -159,6 +159,17 @@ def test_linear_keeps_inf_and_nan_in_their_own_rows(tokens, k, dtype):
     assert bool(got[:, others].isfinite().all())
 
 
+@pytest.mark.parametrize("tokens", [1, 8, 40, 300])
+def test_linear_keeps_subnormal_numbers(tokens):
+    """Subnormal inputs with exact sums, and sums that are subnormal themselves: 64 equal powers of two."""
+    torch, dense = _setup()
+    for dt, low, high in ((torch.float16, -24, 10), (torch.bfloat16, -133, 100), (torch.float16, -14, -15),
+                          (torch.bfloat16, -70, -66)):
+        x = torch.full((tokens, 64), 2.0 ** low, dtype=torch.float64, device="cuda").to(dt)
+        w = torch.full((128, 64), 2.0 ** high, dtype=dt, device="cuda")
+        assert bool((dense.linear(x, w).double() == 64 * 2.0 ** (low + high)).all())
+
+
 # long enough for the largest tiles: a last round cut into halves and a last window of 52 positions, shares of
 # K of the two largest tiles with a partial last step, and a row pitch that is off every 4-byte boundary
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -216,7 +227,8 @@ def _ids(torch, kind, tokens, slots, experts, seed):
 
 EXPERT_SHAPES = [(1, 1, 1, 64, 32), (1, 8, 256, 128, 64), (3, 2, 5, 100, 33), (16, 4, 64, 256, 40), (50, 3, 7, 65, 129),
                  (129, 2, 1000, 64, 48), (400, 6, 24, 136, 200), (900, 2, 3, 72, 260), (700, 1, 1, 64, 520),
-                 (200, 2, 4, 72, 5000), (700, 2, 3, 72, 8200), (1100, 1, 1, 264, 12000), (700, 3, 9, 193, 2600)]
+                 (200, 2, 4, 72, 5000), (700, 2, 3, 72, 8200), (1100, 1, 1, 264, 12000), (700, 3, 9, 193, 2600),
+                 (300, 6, 24, 72, 2300), (300, 6, 24, 67, 2300)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -268,7 +280,8 @@ def test_expert_products_of_whole_numbers_are_exact(tokens, slots, experts, k, n
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("tokens,slots,experts,k,n", [(1, 8, 32, 1024, 96), (2, 8, 32, 1030, 96), (64, 4, 16, 520, 130),
-                                                      (600, 2, 6, 256, 192), (600, 2, 4, 4200, 4160)])
+                                                      (600, 2, 6, 256, 192), (600, 2, 4, 4200, 4160), (300, 6, 24, 264, 1200),
+                                                      (300, 6, 24, 265, 1200)])
 def test_expert_gate_up_and_combine_of_normal_values(tokens, slots, experts, k, n, dtype):
     torch, dense = _setup()
     dt = _dtype(torch, dtype)

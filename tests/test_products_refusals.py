@@ -51,7 +51,7 @@ def test_projection_refusals(change, text):
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(tokens=-1), "negative"), (dict(x=None), "null buffer"), (dict(y=None), "null buffer"), (dict(x=ODD), "odd address"),
+    (dict(tokens=-1), "out of range"), (dict(tokens=(1 << 30) + 1), "out of range"), (dict(x=None), "null buffer"), (dict(y=None), "null buffer"), (dict(x=ODD), "odd address"),
     (dict(y=ODD), "odd address"), (dict(res=ODD, rs=32), "odd address"), (dict(xs=63), "row pitch"), (dict(ys=31), "row pitch"),
     (dict(res=A, rs=31), "row pitch"), (dict(y=A), "must not alias"), (dict(y=C.c_void_p(1 << 22)), "must not alias"),
     (dict(res=B, rs=40), "residual's row pitch")])
@@ -71,7 +71,7 @@ def test_linear_refuses_a_short_workspace():
 
 @pytest.mark.parametrize("kw,text", [
     (dict(experts=0), "expert count"), (dict(experts=1025), "expert count"), (dict(es=2047), "overlap"),
-    (dict(positions=-1), "negative"), (dict(x=None), "null buffer"), (dict(off=None), "null buffer"),
+    (dict(positions=-1), "out of range"), (dict(positions=(1 << 30) + 1, rows=A), "out of range"), (dict(x=None), "null buffer"), (dict(off=None), "null buffer"),
     (dict(y=None), "null buffer"), (dict(x_rows=7), "7 rows for 8"), (dict(x_rows=0, rows=A), "0 rows"),
     (dict(x=ODD), "boundary"), (dict(off=C.c_void_p((1 << 20) + 2)), "boundary"), (dict(xs=8), "row pitch"),
     (dict(ys=8), "row pitch"), (dict(y=A), "must not alias")])
