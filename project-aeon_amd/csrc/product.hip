@@ -78,8 +78,8 @@ __device__ __forceinline__ float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
 
-// Activations in fp32, in place on N values. gelu_tanh is g * sigmoid(2z), as (1 + tanh z) / 2 is
-// sigmoid(2z), without the cancellation. The clamps are comparisons, not fminf/fmaxf: those return
+// Activations in fp32, in place on N values. gelu takes 1 + erf(z) as erfc(-z), and gelu_tanh
+// (1 + tanh z) / 2 as sigmoid(2z): without the cancellation at large negative z. The clamps are comparisons, not fminf/fmaxf: those return
 // the bound for a NaN operand and would turn a NaN pre-activation into a finite value.
 template <int N>
 __device__ __forceinline__ void activate(int kind, float (&g)[N], const float (&u)[N], float limit) {
@@ -90,7 +90,7 @@ __device__ __forceinline__ void activate(int kind, float (&g)[N], const float (&
             break;
         case AEON_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < N; ++i) g[i] *= 0.5f * (1.0f + erff(g[i] * 0.70710678118654752f));
+            for (int i = 0; i < N; ++i) g[i] *= 0.5f * erfcf(g[i] * -0.70710678118654752f);
             break;
         case AEON_ACT_GELU_TANH:
 #pragma unroll
@@ -218,8 +218,10 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& a, int row_blocks, 
         before = __builtin_amdgcn_readlane(before, from);
     }
     const int windows = (held + BM - 1) / BM;
+    const int u = tile - before * row_blocks;
+    if (u < 0 || u >= windows * row_blocks) return false;  // only where they do not, and the sums wrapped
     int window;
-    patch_of(tile - before * row_blocks, windows, row_blocks, &window, &t->row_block);
+    patch_of(u, windows, row_blocks, &window, &t->row_block);
     t->expert = expert;
     t->only = windows == 1;
     t->first = first + window * BM;
@@ -1051,10 +1053,26 @@ __global__ __launch_bounds__(256) void product_combine_kernel(const float* __res
 
 constexpr int kLargestTile = 256;
 
+// A launch counts its threads in 32 bits.
+static int check_grid(long workgroups, int threads) {
+    AEON_REQUIRE(workgroups <= 0xffffffffL / threads, AEON_ERR_INVALID_ARGUMENT,
+                 "product: %ld workgroups are more than one launch holds", workgroups);
+    return AEON_OK;
+}
+
 template <class T, int BM, int BN, int WAVES_M, int WAVES_N, int S, bool ALIGNED>
 static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
     auto kernel = product_kernel<T, BM, BN, WAVES_M, WAVES_N, S, ALIGNED>;
     constexpr int bytes = S * (BM + BN) * kStepBytes;
+    const long rows = a.pair ? BN / 2 : BN;
+    const long row_blocks = (a.n + rows - 1) / rows;
+    // an upper bound of the windows: every list that holds something may end in a short one
+    long windows = (static_cast<long>(a.positions) + BM - 1) / BM;
+    if (a.offsets != nullptr) windows = a.positions / BM + (a.experts < a.positions ? a.experts : a.positions);
+    long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
+    // room for a last round in halves
+    if (takes_turns(BM, ALIGNED) && a.offsets == nullptr) grid += kXcds * (kXcdCus / 2);
+    if (int rc = check_grid(grid, 64 * WAVES_M * WAVES_N)) return rc;
     if (bytes > 65536) {
         // more dynamic LDS than the default limit has to be asked for, once per kernel and device
         static std::atomic<uint64_t> raised{0};
@@ -1067,15 +1085,6 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
             raised.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    const long rows = a.pair ? BN / 2 : BN;
-    const long row_blocks = (a.n + rows - 1) / rows;
-    // an upper bound of the windows: every list that holds something may end in a short one
-    long windows = (static_cast<long>(a.positions) + BM - 1) / BM;
-    if (a.offsets != nullptr) windows = a.positions / BM + (a.experts < a.positions ? a.experts : a.positions);
-    long grid = (windows * row_blocks + kXcds - 1) / kXcds * kXcds;
-    // room for a last round in halves
-    if (takes_turns(BM, ALIGNED) && a.offsets == nullptr) grid += kXcds * (kXcdCus / 2);
-    AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
     kernel<<<dim3(static_cast<unsigned>(grid), splits), 64 * WAVES_M * WAVES_N, bytes, stream>>>(a);
     AEON_LAUNCH_CHECK();
     return AEON_OK;
@@ -1086,7 +1095,7 @@ static int launch_tile(const ProductArgs& a, int splits, hipStream_t stream) {
 template <class T, int ROWS, int MATS>
 static int launch_few_rows(const ProductArgs& a, long windows, hipStream_t stream) {
     const long grid = (windows * ((a.n + ROWS - 1) / ROWS) + kXcds - 1) / kXcds * kXcds;
-    AEON_REQUIRE(grid <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "product: %ld workgroups are more than one launch holds", grid);
+    if (int rc = check_grid(grid, 64 * kFewWaves)) return rc;
     product_few_kernel<T, ROWS, MATS><<<static_cast<unsigned>(grid), 64 * kFewWaves, 0, stream>>>(a);
     AEON_LAUNCH_CHECK();
     return AEON_OK;
@@ -1418,10 +1427,10 @@ extern "C" int aeon_expert_combine(const aeon_projection* projection, int expert
         AEON_LAUNCH_CHECK();
         return AEON_OK;
     }
-    if (int rc = launch_product(w.dtype, plan_experts(w, a.positions, experts), a, 1, as_stream(stream))) return rc;
     const int row_blocks = (w.out_dim + 1023) / 1024;
     const long blocks = static_cast<long>(tokens) * row_blocks;
-    AEON_REQUIRE(blocks <= 0x7fffffffL, AEON_ERR_INVALID_ARGUMENT, "%s: too many outputs for one launch", who);
+    if (int rc = check_grid(blocks, 256)) return rc;
+    if (int rc = launch_product(w.dtype, plan_experts(w, a.positions, experts), a, 1, as_stream(stream))) return rc;
     const auto grid = static_cast<unsigned>(blocks);
     if (w.dtype == AEON_DTYPE_F16) {
         product_combine_kernel<F16><<<grid, 256, 0, as_stream(stream)>>>(a.wide, d_topk_ids, experts, row_blocks, slots, w.out_dim,

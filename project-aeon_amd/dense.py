@@ -177,7 +177,8 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
 def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None, out=None):
     """base + the weighted sum of each token's expert products, in slot order (aeon_expert_combine).
     h [tokens * slots][in_dim] by position, weight [experts][out_dim][in_dim], ids int32 and weights fp32
-    [tokens][slots]. Returns [tokens][out_dim]; `out` may be the base itself."""
+    [tokens][slots], offsets and draws the lists of these ids: a draw is left out by an id outside
+    [0, experts), not by taking it from a list. Returns [tokens][out_dim]; `out` may be the base itself."""
     p = _projection(h, weight, bias, "none", None, None, 0.0, 1)
     if ids.dim() != 2:
         raise ValueError("ids has to be [tokens][slots]")

@@ -159,6 +159,26 @@ def test_linear_keeps_inf_and_nan_in_their_own_rows(tokens, k, dtype):
     assert bool(got[:, others].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_activations_far_from_zero(act, dtype):
+    """act(g) of exact g from -14 to 14 (g times a one in the first column), element by element: half a step of
+    the type, plus what fp32 loses: an argument z of an exponential, rounded in a few operations, moves the
+    exponential by a few |z| * 2^-24 of itself, and the rest is at most 16 units of 2^-23. What is below the
+    type's smallest step, or 2^-120 in fp32, may be lost."""
+    torch, dense = _setup()
+    dt = _dtype(torch, dtype)
+    g = torch.linspace(-14, 14, 3601, dtype=torch.float64, device="cuda").to(dt)
+    x, w = torch.zeros(g.numel(), 64, dtype=dt, device="cuda"), torch.zeros(16, 64, dtype=dt, device="cuda")
+    x[:, 0], w[:, 0] = g, 1.0
+    got, g = dense.linear(x, w, activation=act), g.double()
+    z = {"silu": g, "gelu": g * g / 2, "gelu_tanh": 2 * (2 / np.pi) ** 0.5 * (g + 0.044715 * g ** 3)}[act]
+    want = 0.5 * g * torch.special.erfc(-g * 0.5 ** 0.5) if act == "gelu" else g * torch.special.expit(z)
+    loss = want.abs() * (4 * z.abs() + 16) * 2.0 ** -23
+    least = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2 if dtype == "f16" else 2.0 ** -120
+    _near(torch, got, want[:, None].expand_as(got), (loss + least)[:, None])
+
+
 @pytest.mark.parametrize("tokens", [1, 8, 40, 300])
 def test_linear_keeps_subnormal_numbers(tokens):
     """Subnormal inputs with exact sums, and sums that are subnormal themselves: 64 equal powers of two."""

@@ -117,3 +117,13 @@ def test_the_tensor_functions_check_their_operands():
     with pytest.raises(ValueError, match="hidden"):
         from project_aeon_amd import moe
         moe.UnquantisedMoeLayer(torch.zeros(2, 3, 4), torch.zeros(2, 3, 4), torch.zeros(2, 3, 4), 1, 7.0)
+
+
+def test_calls_of_more_threads_than_a_launch_holds():
+    wide = dict(out_dim=1 << 24)
+    calls = (lambda: _linear(_p(out_dim=1 << 20), tokens=1 << 30, ys=1 << 20),
+             lambda: _experts(_p(**wide), experts=64, es=1 << 30, positions=16, x_rows=16, ys=1 << 24),
+             lambda: _combine(_p(), tokens=1 << 25, slots=1, wb=1 << 40))
+    for call in calls:
+        with pytest.raises(ValueError, match="more than one launch holds"):
+            call()
