@@ -1051,7 +1051,9 @@ __global__ __launch_bounds__(256) void product_combine_kernel(const float* __res
 
 // ---- launches --------------------------------------------------------------------------------
 
-constexpr int kLargestTile = 256;
+// Tiles, positions x weight rows. 128 x 128 is there twice: two workgroups of two stages a CU, for
+// many tiles, or one of four stages and twice the waves.
+enum Tile : int { kTileFew, kTile16x64, kTile32x64, kTile32x32, kTile64x64, kTile64x32, kTile128Pair, kTile128Alone, kTile256 };
 
 // A launch counts its threads in 32 bits.
 static int check_grid(long workgroups, int threads) {
@@ -1112,20 +1114,25 @@ static int launch_few(const ProductArgs& a, hipStream_t stream) {
 }
 
 template <class T, bool ALIGNED>
-static int launch_tiles(int tile, const ProductArgs& a, int splits, hipStream_t stream) {
+static int launch_tiles(Tile tile, const ProductArgs& a, int splits, hipStream_t stream) {
     if constexpr (ALIGNED) {
         switch (tile) {
-            case 16: return launch_tile<T, 16, 64, 1, 2, 7, true>(a, splits, stream);
-            case 32: return launch_tile<T, 32, 64, 1, 2, 6, true>(a, splits, stream);
-            case 64: return launch_tile<T, 64, 64, 2, 2, 5, true>(a, splits, stream);
-            case 128: return launch_tile<T, 128, 128, 2, 2, 2, true>(a, splits, stream);
+            case kTile16x64: return launch_tile<T, 16, 64, 1, 2, 7, true>(a, splits, stream);
+            case kTile32x64: return launch_tile<T, 32, 64, 1, 2, 6, true>(a, splits, stream);
+            case kTile32x32: return launch_tile<T, 32, 32, 2, 1, 9, true>(a, splits, stream);
+            case kTile64x64: return launch_tile<T, 64, 64, 2, 2, 5, true>(a, splits, stream);
+            case kTile64x32: return launch_tile<T, 64, 32, 4, 1, 6, true>(a, splits, stream);
+            case kTile128Pair: return launch_tile<T, 128, 128, 2, 2, 2, true>(a, splits, stream);
+            case kTile128Alone: return launch_tile<T, 128, 128, 2, 4, 4, true>(a, splits, stream);
             default: return launch_tile<T, 256, 256, 2, 4, 2, true>(a, splits, stream);
         }
     } else {
         switch (tile) {
-            case 16:
-            case 32: return launch_tile<T, 32, 64, 1, 2, 2, false>(a, splits, stream);
-            case 64: return launch_tile<T, 64, 64, 2, 2, 2, false>(a, splits, stream);
+            case kTile16x64:
+            case kTile32x64:
+            case kTile32x32: return launch_tile<T, 32, 64, 1, 2, 2, false>(a, splits, stream);
+            case kTile64x64:
+            case kTile64x32: return launch_tile<T, 64, 64, 2, 2, 2, false>(a, splits, stream);
             default: return launch_tile<T, 128, 128, 2, 2, 2, false>(a, splits, stream);
         }
     }
@@ -1133,10 +1140,10 @@ static int launch_tiles(int tile, const ProductArgs& a, int splits, hipStream_t 
 
 static bool on_boundary(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipStream_t stream) {
+static int launch_product(int dtype, Tile tile, ProductArgs& a, int splits, hipStream_t stream) {
     const bool aligned = on_boundary(a.x, 4) && on_boundary(a.w[0], 4) && on_boundary(a.w[1], 4) && a.x_stride % 2 == 0 &&
                          a.w_stride % 2 == 0 && a.expert_stride % 2 == 0;
-    if (tile == kFewMax) return dtype == AEON_DTYPE_F16 ? launch_few<F16>(a, stream) : launch_few<BF16>(a, stream);
+    if (tile == kTileFew) return dtype == AEON_DTYPE_F16 ? launch_few<F16>(a, stream) : launch_few<BF16>(a, stream);
     if (dtype == AEON_DTYPE_F16) {
         return aligned ? launch_tiles<F16, true>(tile, a, splits, stream) : launch_tiles<F16, false>(tile, a, splits, stream);
     }
@@ -1145,57 +1152,61 @@ static int launch_product(int dtype, int tile, ProductArgs& a, int splits, hipSt
 
 constexpr int kMostPositions = 1 << 30;  // positions and their sums with a tile's are 32-bit numbers
 
-// Positions a tile holds and the shares K is cut into.
+// A tile and the shares K is cut into.
 struct ProductPlan {
-    int tile, splits, split_steps;
+    Tile tile;
+    int splits, split_steps;
 };
 
 // What a tile costs, us: a 64-column step of a workgroup that has its CU to itself, of one of two that
-// share it, and the rest of a workgroup (launch, first requests, epilogue). Fitted to products of
-// 5 to 4096 tokens with matrices of 512 x 1024 to 7168 x 7168, each at every tile and at one to eight
-// shares, weights cold (72 products; the plan made from these figures is within 1.2 % of the best one
-// measured in the mean, and 18 % at worst).
+// share it (0: it never does), and the rest of a workgroup (launch, first requests, epilogue). Fitted to
+// products of 5 to 4096 tokens with matrices of 512 x 1024 to 7168 x 7168, each at every tile and at one to
+// eight shares, weights cold (120 products; the plan made from these figures is within 0.3 % of the best one
+// measured in the mean, and 7 % at worst).
+// Without the tiles of 32 rows and the 128 x 128 one that has its CU alone the same products take 6 % more in
+// the mean: 128 tokens, K 2048, N 4096: 12.5 us, 10.7 with 64 x 32; 512 tokens, K = N = 7168: 82, and 69 with 128 x 128.
 struct TileCost {
+    Tile tile;
     int positions, rows;
     double step_alone, step_shared, fixed;
 };
-constexpr TileCost kTileCosts[] = {{16, 64, 0.12, 0.27, 2.8}, {32, 64, 0.16, 0.34, 3.0}, {64, 64, 0.21, 0.40, 2.9},
-                                   {128, 128, 0.68, 1.04, 4.1}, {kLargestTile, kLargestTile, 1.38, 0.0, 18.8}};
+constexpr TileCost kTileCosts[] = {{kTile32x32, 32, 32, 0.12, 0.29, 2.2}, {kTile64x32, 64, 32, 0.12, 0.27, 2.2},
+                                   {kTile64x64, 64, 64, 0.19, 0.39, 3.0}, {kTile128Alone, 128, 128, 0.46, 0.0, 8.1},
+                                   {kTile256, 256, 256, 1.43, 0.0, 16.0}};
 
 // Every tile and number of shares priced: rounds of workgroups, the weights' way from memory, and the
 // second launch that joins shares with its traffic.
 static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
-    if (tokens <= kFewMax && w.in_dim >= kFewColumns) return ProductPlan{kFewMax, 1, 0};
+    if (tokens <= kFewMax && w.in_dim >= kFewColumns) return ProductPlan{kTileFew, 1, 0};
     const double n = static_cast<double>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     const int steps = (w.in_dim + kStep - 1) / kStep;
-    const double stream = (n + tokens) * w.in_dim * 2 / 9.3e6 + 2.7;
-    ProductPlan best{16, 1, steps};
+    const double stream = (n + tokens) * w.in_dim * 2 / 9.7e6 + 3.6;
+    ProductPlan best{kTile64x64, 1, steps};
     double best_us = 0.0;
     for (const TileCost& t : kTileCosts) {
-        if (t.positions > 64 ? t.positions > 2L * tokens : t.positions < 64 && t.positions * 4L < tokens) continue;
+        // tiles that would stay half empty, or be far too many
+        if (t.positions > 64 ? t.positions > 2L * tokens : t.rows < 64 && (t.positions < 64 ? tokens > 128 : tokens > 512)) continue;
         const double tiles = static_cast<double>((tokens + t.positions - 1) / t.positions) *
                              ((static_cast<long>(n) + t.rows - 1) / t.rows);
         for (int splits : {1, 2, 3, 4, 6, 8}) {
             if (splits > 1 && (splits > steps / 2 || tiles * splits > 1100)) break;
             const int each = (steps + splits - 1) / splits;
             const long groups = static_cast<long>(tiles * splits);
-            double us;
-            if (t.positions == kLargestTile) {
-                const long last = groups % 256;
-                const double half = 0.55;  // of a tile's products, where its positions or its last round fill one half
-                us = groups / 256 * (each * t.step_alone + t.fixed);
-                if (last > 0) us += each * t.step_alone * (last <= 128 && splits == 1 && tokens > 128 ? half : 1.0) + t.fixed;
-                if (tokens <= 128) us *= half;
-            } else {
-                const long last = groups % 512;
-                us = groups / 512 * (each * t.step_shared + t.fixed);
-                if (last > 0) us += each * (last <= 256 ? t.step_alone : t.step_shared) + t.fixed;
+            const int round = t.step_shared > 0.0 ? 512 : 256;
+            const long last = groups % round;
+            double us = groups / round * (each * (t.step_shared > 0.0 ? t.step_shared : t.step_alone) + t.fixed);
+            if (last > 0) {
+                double step = last <= 256 ? t.step_alone : t.step_shared;
+                // a last round of the waves that take turns is cut into halves of 0.55 of a tile's products
+                if (t.tile == kTile256 && last <= 128 && splits == 1 && tokens > 128) step *= 0.55;
+                us += each * step + t.fixed;
             }
+            if (t.tile == kTile256 && tokens <= 128) us *= 0.55;
             if (us < stream) us = stream;
-            if (splits > 1) us += 1.3 + 8.0 * splits * tokens * n / 11e6;
+            if (splits > 1) us += 0.7 + 8.0 * splits * tokens * n / 14.5e6;
             if (best_us == 0.0 || us < best_us) {
                 best_us = us;
-                best = ProductPlan{t.positions, splits, each};
+                best = ProductPlan{t.tile, splits, each};
             }
         }
     }
@@ -1209,16 +1220,16 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
 // 64: 168 / 189 / 262 / 306 / 361 / 489; 128: 185 / 202 / 221 / 240 / 288 / 356; 256: 204 / 207 / 214 / 219 /
 // 234 / 273. Gated, 2048 outputs of 4096 columns, at 64 / 96 / 128: 128: 385 / 403 / 528, 256: 408 / 405 /
 // 428. Eight experts of 4096 x 4096, tile 64 / 128 / 256, at 96: 66 / 72 / 66; at 192: 106 / 76 / 87; at 256:
-// 146 / 131 / 92.
-static int plan_experts(const aeon_projection& w, int positions, int experts) {
-    if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kFewMax;
+// 146 / 131 / 92; tile 32 / 64 at 24: 57 / 49. Tiles of 32 rows, 8 positions in 64 of 4096 x 2048: 190 to 216.
+static Tile plan_experts(const aeon_projection& w, int positions, int experts) {
+    if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kTileFew;
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
     const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
-    if (mean > 80 && tiles(kLargestTile) >= 192) return kLargestTile;
-    if (mean > 48 && tiles(128) >= 400) return 128;
-    return mean <= 12 ? 16 : mean <= 24 ? 32 : 64;
+    if (mean > 80 && tiles(256) >= 192) return kTile256;
+    if (mean > 48 && tiles(128) >= 400) return kTile128Pair;
+    return mean <= 12 ? kTile16x64 : mean <= 20 ? kTile32x64 : kTile64x64;
 }
 
 static int check_projection(const aeon_projection* w, const char* who) {
