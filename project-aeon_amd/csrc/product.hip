@@ -18,7 +18,7 @@
 //
 // What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
 //   4 x any    the weight stream, by registers and VALU: 6.3 TB/s over the eight experts of one token
-//   16..64     the weight stream while it is long: 7.0 TB/s over 12.9 GB (64 tokens, 256 experts); in
+//   16..64     the weight stream while it is long: 6.8 TB/s over 12.9 GB (64 tokens, 256 experts); in
 //              short products a workgroup's own start and end, and with 64 positions LDS and the way
 //              from L2 to it (about 80 GB/s a CU)
 //   128, 256   the matrix pipe: a 256 x 256 x 64 step takes 1.36 us where the panels are in L2, 1.58
@@ -1160,7 +1160,7 @@ struct ProductPlan {
 
 // What a tile costs, us: a 64-column step of a workgroup that has its CU to itself, of one of two that
 // share it (0: it never does), and the rest of a workgroup (launch, first requests, epilogue). Fitted to
-// products of 5 to 4096 tokens with matrices of 512 x 1024 to 7168 x 7168, each at every tile and at one to
+// products of 5 to 4096 tokens with matrices of 1024 x 512 to 14336 x 4096, each at every tile and at one to
 // eight shares, weights cold (120 products; the plan made from these figures is within 0.3 % of the best one
 // measured in the mean, and 7 % at worst).
 // Without the tiles of 32 rows and the 128 x 128 one that has its CU alone the same products take 6 % more in
