@@ -466,8 +466,8 @@ int aeon_expert_linear(const aeon_projection* projection, int experts, long expe
  * position whose draw_indices[p] is t*slots + s, and e = ids[t][s] the expert that lists it. Every
  * draw whose id is in [0, experts) has to be in that expert's list, as the permutation makes them
  * (to leave a draw out, give it an id outside that range before the permutation); a slot whose id is
- * outside contributes nothing. The contributions stay fp32 (in the workspace, 16-byte boundary; a token
- * or two need none). d_base is nullable and may be d_out (same pitch). The projection has no
+ * outside contributes nothing. The contributions stay fp32 (in the workspace, 16-byte boundary; a
+ * few tokens need none). d_base is nullable and may be d_out (same pitch). The projection has no
  * activation. d_h has tokens * slots rows, by position. */
 size_t aeon_expert_combine_workspace_bytes(const aeon_projection* projection, int tokens, int slots);
 int aeon_expert_combine(const aeon_projection* projection, int experts, long expert_stride,

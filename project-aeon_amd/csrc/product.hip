@@ -17,7 +17,7 @@
 // so both pre-activations of an output meet in one lane.
 //
 // What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
-//   4 x any    the weight stream, by registers and VALU: 6.3 TB/s over the eight experts of one token
+//   4 x any    launch and a trip to memory (1 token, 4096 -> 256: 3.4 us), and the FMAs from two positions on
 //   16..64     the weight stream while it is long: 6.8 TB/s over 12.9 GB (64 tokens, 256 experts); in
 //              short products a workgroup's own start and end, and with 64 positions LDS and the way
 //              from L2 to it (about 80 GB/s a CU)
@@ -807,6 +807,7 @@ __device__ __forceinline__ void row_dots(const uint16_t* const (&w)[R], const ui
 constexpr int kFewWaves = 4;
 constexpr int kFewMax = 4;  // positions of a window
 constexpr int kFewColumns = 8;
+constexpr int kFewTokens = 16;  // of a dense product that may still be cheapest in a few such windows
 
 template <class T, int ROWS, int MATS, int TOK>
 __device__ __forceinline__ void few_body(const ProductArgs& a, const ProductTile& t, float (*sums)[kFewWaves]) {
@@ -877,11 +878,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(const Produ
 
 // The weighted sum of a token's expert products in one launch: a workgroup walks the slots of its
 // token for ROWS outputs, so nothing passes through memory between the products and the sum. Every
-// slot streams its expert's rows anew, hence for a token or two. The slots' chunks of K follow each
+// slot streams its expert's rows anew, hence for a few tokens. The slots' chunks of K follow each
 // other in one sequence whose next loads are issued before the present ones are used. At most 64
-// draws: lane l holds draw l's id, weight and position.
+// draws: lane l holds draw l's id, weight and position. Measured, us of this kernel / of two launches: 3 tokens of
+// 8 slots, 2048 -> 7168: 108 / 115; 8 tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.0 / 16.7; 12 tokens (50 MB): 13.5
+// / 10.3; 4 tokens of 6 slots, 512 -> 2048 (50 MB): 12.3 / 16.7, 6 tokens (75 MB): 19.8 / 19.0.
 constexpr int kDirectDraws = 64;
-constexpr int kDirectTokens = 2;
+constexpr int kDirectTokens = 3;
+constexpr double kDirectBytes = 40e6;  // rows streamed, above which more tokens go through memory
 template <class T, int ROWS>
 __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const ProductArgs a, const int32_t* ids, int slots,
                                                                        const uint16_t* base, long base_stride,
@@ -1175,14 +1179,20 @@ constexpr TileCost kTileCosts[] = {{kTile32x32, 32, 32, 0.12, 0.29, 2.2}, {kTile
                                    {kTile256, 256, 256, 1.43, 0.0, 16.0}};
 
 // Every tile and number of shares priced: rounds of workgroups, the weights' way from memory, and the
-// second launch that joins shares with its traffic.
+// second launch that joins shares with its traffic. The kernel for a few positions pays by eight
+// weight rows: what a workgroup costs beside its loads, more with the FMAs of two or four positions. Measured,
+// us in it / in the best tile: 1 token, 4096 -> 256: 3.4 / 8.5, 7168 -> 7168: 21.1 / 22.6, 512 -> 32000: 18.8 / 9.2;
+// 4 tokens: 4.5 / 8.6, 26.5 / 21.1, 45.6 / 9.3; 8 tokens, 4096 -> 256: 4.7 / 9.0.
 static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
-    if (tokens <= kFewMax && w.in_dim >= kFewColumns) return ProductPlan{kTileFew, 1, 0};
     const double n = static_cast<double>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
     const int steps = (w.in_dim + kStep - 1) / kStep;
     const double stream = (n + tokens) * w.in_dim * 2 / 9.7e6 + 3.6;
-    ProductPlan best{kTile64x64, 1, steps};
+    ProductPlan best{kTileFew, 1, steps};
     double best_us = 0.0;
+    if (tokens <= kFewTokens && w.in_dim >= kFewColumns) {
+        const double each = (tokens == 1 ? 2.5e-3 : tokens == 2 ? 4.7e-3 : 8.5e-3) + 1.65e-6 * w.in_dim;
+        best_us = 1.4 + n / 8 * ((tokens + kFewMax - 1) / kFewMax) * each;
+    }
     for (const TileCost& t : kTileCosts) {
         // tiles that would stay half empty, or be far too many
         if (t.positions > 64 ? t.positions > 2L * tokens : t.rows < 64 && (t.positions < 64 ? tokens > 128 : tokens > 512)) continue;
@@ -1214,7 +1224,10 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
     return best;
 }
 
-// Lists: by how many positions an expert holds on average, and only as large a tile as leaves the CUs
+// Lists. A few positions with small matrices: the kernel that has no ring. Measured, us in it / in 16 x 64 tiles:
+// 4 draws over 8 experts of 1024 x 1024: 7.0 / 8.0, 8 draws 13.5 / 8.2; 2 draws of 4096 x 4096: 15.8 / 19.3, 4 draws:
+// 28.0 / 28.7; 4 draws of 4096 x 1024: 14.9 / 9.2; 8 gated draws of 2048 x 7168: 76 / 73.
+// Otherwise by how many positions an expert holds on average, and only as large a tile as leaves the CUs
 // enough of them (half a window an expert is taken to be short). Measured, us per product at a mean of 16 /
 // 32 / 64 / 96 / 128 / 192 positions, 64 experts of 4096 x 2048: tile 32: 172 / 222 / 316 / 407 / 498 / 689;
 // 64: 168 / 189 / 262 / 306 / 361 / 489; 128: 185 / 202 / 221 / 240 / 288 / 356; 256: 204 / 207 / 214 / 219 /
@@ -1222,10 +1235,10 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
 // 428. Eight experts of 4096 x 4096, tile 64 / 128 / 256, at 96: 66 / 72 / 66; at 192: 106 / 76 / 87; at 256:
 // 146 / 131 / 92; tile 32 / 64 at 24: 57 / 49. Tiles of 32 rows, 8 positions in 64 of 4096 x 2048: 190 to 216.
 static Tile plan_experts(const aeon_projection& w, int positions, int experts) {
-    if ((positions <= 16 || positions <= experts / 16) && w.in_dim >= kFewColumns) return kTileFew;
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
     const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
+    if (mean <= kFewMax && live * n <= (positions <= 4 ? 8192 : 6144) && w.in_dim >= kFewColumns) return kTileFew;
     auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
     if (mean > 80 && tiles(256) >= 192) return kTile256;
     if (mean > 48 && tiles(128) >= 400) return kTile128Pair;
@@ -1281,7 +1294,9 @@ static int check_experts(const aeon_projection& w, int experts, long expert_stri
 }
 
 static bool combine_direct(const aeon_projection& w, int tokens, int slots) {
-    return tokens <= kDirectTokens && static_cast<long>(tokens) * slots <= kDirectDraws && w.in_dim >= kFewColumns;
+    const long draws = static_cast<long>(tokens) * slots;
+    return draws <= kDirectDraws && w.in_dim >= kFewColumns &&
+           (tokens <= kDirectTokens || 2.0 * draws * w.in_dim * w.out_dim <= kDirectBytes);
 }
 
 static int check_workspace(const void* d_workspace, size_t bytes, size_t need, const char* who) {

@@ -86,7 +86,7 @@ def test_expert_linear_refusals(kw, text):
     (dict(draws=None), "null buffer"), (dict(ids=None), "null buffer"), (dict(w=None), "null buffer"),
     (dict(out=None), "null buffer"), (dict(h=ODD), "boundary"), (dict(w=C.c_void_p(2)), "boundary"), (dict(hs=1), "row pitch"),
     (dict(os=1), "row pitch"), (dict(base=A, bs=1), "row pitch"), (dict(out=A), "must not alias"),
-    (dict(base=B, bs=40), "base's row pitch"), (dict(ws=None), "workspace of"), (dict(wb=8), "workspace of")])
+    (dict(base=B, bs=40), "base's row pitch"), (dict(tokens=40, ws=None), "workspace of"), (dict(tokens=40, wb=8), "workspace of")])
 def test_expert_combine_refusals(kw, text):
     with pytest.raises(ValueError, match=text):
         _combine(_p(), **kw)
@@ -122,7 +122,7 @@ def test_the_tensor_functions_check_their_operands():
 def test_calls_of_more_threads_than_a_launch_holds():
     wide = dict(out_dim=1 << 24)
     calls = (lambda: _linear(_p(out_dim=1 << 20), tokens=1 << 30, ys=1 << 20),
-             lambda: _experts(_p(**wide), experts=64, es=1 << 30, positions=16, x_rows=16, ys=1 << 24),
+             lambda: _experts(_p(**wide), experts=1024, es=1 << 30, positions=1024, x_rows=1024, ys=1 << 24),
              lambda: _combine(_p(), tokens=1 << 25, slots=1, wb=1 << 40))
     for call in calls:
         with pytest.raises(ValueError, match="more than one launch holds"):
