@@ -880,9 +880,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(const Produ
 // token for ROWS outputs, so nothing passes through memory between the products and the sum. Every
 // slot streams its expert's rows anew, hence for a few tokens. The slots' chunks of K follow each
 // other in one sequence whose next loads are issued before the present ones are used. At most 64
-// draws: lane l holds draw l's id, weight and position. Measured, us of this kernel / of two launches: 3 tokens of
-// 8 slots, 2048 -> 7168: 108 / 115; 8 tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.0 / 16.7; 12 tokens (50 MB): 13.5
-// / 10.3; 4 tokens of 6 slots, 512 -> 2048 (50 MB): 12.3 / 16.7, 6 tokens (75 MB): 19.8 / 19.0.
+// draws: lane l holds draw l's id, weight and position. Measured, us of this kernel / of two launches: 1 and 3 tokens of
+// 8 slots, 2048 -> 7168: 41.8 / 48.6 and 108 / 109; 8 tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.2 / 10.3; 12 tokens
+// (50 MB): 13.5 / 10.3; 4 tokens of 6 slots, 512 -> 2048 (50 MB): 13.3 / 16.5, 6 tokens (75 MB): 19.6 / 18.7. The host
+// spends 4 us less on it.
 constexpr int kDirectDraws = 64;
 constexpr int kDirectTokens = 3;
 constexpr double kDirectBytes = 40e6;  // rows streamed, above which more tokens go through memory
@@ -1226,7 +1227,8 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
 
 // Lists. A few positions with small matrices: the kernel that has no ring. Measured, us in it / in 16 x 64 tiles:
 // 4 draws over 8 experts of 1024 x 1024: 7.0 / 8.0, 8 draws 13.5 / 8.2; 2 draws of 4096 x 4096: 15.8 / 19.3, 4 draws:
-// 28.0 / 28.7; 4 draws of 4096 x 1024: 14.9 / 9.2; 8 gated draws of 2048 x 7168: 76 / 73.
+// 28.0 / 28.7; 4 draws of 4096 x 1024: 14.9 / 9.2; 16 draws over 256 of 256 x 1024: 7.8 / 8.7, over 8 of 256 x 128
+// (two or three positions an expert): 9.8 / 7; 8 gated draws of 2048 x 7168: 76 / 73.
 // Otherwise by how many positions an expert holds on average, and only as large a tile as leaves the CUs
 // enough of them (half a window an expert is taken to be short). Measured, us per product at a mean of 16 /
 // 32 / 64 / 96 / 128 / 192 positions, 64 experts of 4096 x 2048: tile 32: 172 / 222 / 316 / 407 / 498 / 689;
@@ -1238,7 +1240,8 @@ static Tile plan_experts(const aeon_projection& w, int positions, int experts) {
     const int live = experts < positions ? experts : positions;
     const int mean = positions / (live > 0 ? live : 1);
     const long n = static_cast<long>(w.out_dim) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1);
-    if (mean <= kFewMax && live * n <= (positions <= 4 ? 8192 : 6144) && w.in_dim >= kFewColumns) return kTileFew;
+    const bool spread = 2L * positions <= experts;  // mostly one position an expert
+    if ((positions <= 4 ? live * n <= 8192 : spread && live * n <= 6144) && w.in_dim >= kFewColumns) return kTileFew;
     auto tiles = [&](long tile) { return (positions / tile + (live + 1) / 2) * ((n + tile - 1) / tile); };
     if (mean > 80 && tiles(256) >= 192) return kTile256;
     if (mean > 48 && tiles(128) >= 400) return kTile128Pair;

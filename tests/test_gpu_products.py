@@ -248,7 +248,8 @@ def _ids(torch, kind, tokens, slots, experts, seed):
 EXPERT_SHAPES = [(1, 1, 1, 64, 32), (1, 8, 256, 128, 64), (3, 2, 5, 100, 33), (16, 4, 64, 256, 40), (50, 3, 7, 65, 129),
                  (129, 2, 1000, 64, 48), (400, 6, 24, 136, 200), (900, 2, 3, 72, 260), (700, 1, 1, 64, 520),
                  (200, 2, 4, 72, 5000), (700, 2, 3, 72, 8200), (1100, 1, 1, 264, 12000), (700, 3, 9, 193, 2600),
-                 (300, 6, 24, 72, 2300), (300, 6, 24, 67, 2300), (33, 2, 66, 128, 64), (8, 1, 9, 4104, 680)]
+                 (300, 6, 24, 72, 2300), (300, 6, 24, 67, 2300), (33, 2, 140, 128, 64), (8, 1, 16, 4104, 680),
+                 (33, 2, 66, 128, 64), (8, 1, 9, 4104, 680)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
