@@ -33,14 +33,10 @@ class Projection(C.Structure):
 # reads, and one call costs the host about as much as one of torch's own element-wise operators.
 
 
-def _fits(t, device, dtype, shape):
-    """Of this type, on this GPU, of this shape, the elements of a row next to each other."""
-    return (t.dtype is dtype and t.get_device() == device and t.shape == shape
-            and (t.stride(-1) == 1 or t.shape[-1] <= 1))
-
-
 def _check(t, name, device, dtype, shape):
-    if _fits(t, device, dtype, shape):
+    """Of this type, on this GPU, of this shape, the elements of a row next to each other."""
+    if (t.dtype is dtype and t.get_device() == device and t.shape == shape
+            and (t.stride(-1) == 1 or shape[-1] <= 1)):
         return
     if t.dtype is not dtype:
         raise ValueError("%s is %s, not %s" % (name, t.dtype, dtype))
@@ -94,14 +90,16 @@ def _check_bias(b, name, device, kind, shape):
         raise ValueError("%s has to be contiguous" % name)
 
 
-def _call(device, name, *args):
+def _call(device, entry, *args):
     """One entry point on the current stream of a GPU, with that GPU current."""
     stream = torch._C._cuda_getCurrentRawStream(device)
-    if device == torch.cuda.current_device():
-        capi.call(name, *args, stream)
+    if device == torch._C._cuda_getDevice():
+        rc = entry(*args, stream)
     else:
         with torch.cuda.device(device):
-            capi.call(name, *args, stream)
+            rc = entry(*args, stream)
+    if rc != capi.OK:
+        capi.check(rc)
 
 
 def _output(out, x, shape):
@@ -125,10 +123,10 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
     if residual is not None:
         _check(residual, "residual", device, x.dtype, shape)
     out = _output(out, x, shape)
-    at = C.addressof(p)
-    need = capi.lib().aeon_linear_workspace_bytes(at, tokens)
+    at, lib = C.addressof(p), capi.lib()
+    need = lib.aeon_linear_workspace_bytes(at, tokens)
     ws = _workspace(x, need)
-    _call(device, "aeon_linear", at, x.data_ptr(), _pitch(x), tokens, _ptr(residual),
+    _call(device, lib.aeon_linear, at, x.data_ptr(), _pitch(x), tokens, _ptr(residual),
           0 if residual is None else _pitch(residual), out.data_ptr(), _pitch(out), _ptr(ws), need)
     return out
 
@@ -169,7 +167,7 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
     positions = x_rows if rows is None else rows.shape[0]
     _lists(device, weight.shape[0], offsets, positions, rows, "rows")
     out = _output(out, x, (positions, p.out_dim))
-    _call(device, "aeon_expert_linear", C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), _pitch(x),
+    _call(device, capi.lib().aeon_expert_linear, C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), _pitch(x),
           x_rows, offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), _pitch(out))
     return out
 
@@ -195,10 +193,10 @@ def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None
     if base is not None:
         _check(base, "base", device, h.dtype, shape)
     out = _output(out, h, shape)
-    at = C.addressof(p)
-    need = capi.lib().aeon_expert_combine_workspace_bytes(at, tokens, slots)
+    at, lib = C.addressof(p), capi.lib()
+    need = lib.aeon_expert_combine_workspace_bytes(at, tokens, slots)
     ws = _workspace(h, need)
-    _call(device, "aeon_expert_combine", at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), _pitch(h),
+    _call(device, lib.aeon_expert_combine, at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), _pitch(h),
           offsets.data_ptr(), draws.data_ptr(), ids.data_ptr(), weights.data_ptr(), tokens, slots, _ptr(base),
           0 if base is None else _pitch(base), out.data_ptr(), _pitch(out), _ptr(ws), need)
     return out
