@@ -18,7 +18,7 @@
 //
 // What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
 //   4 x any    launch and a trip to memory (1 token, 4096 -> 256: 3.4 us), and the FMAs from two positions on
-//   16..64     the weight stream while it is long: 6.8 TB/s over 12.9 GB (64 tokens, 256 experts); in
+//   16..64     the weight stream while it is long: 6.9 TB/s over 12.9 GB (64 tokens, 256 experts); in
 //              short products a workgroup's own start and end, and with 64 positions LDS and the way
 //              from L2 to it (about 80 GB/s a CU)
 //   128, 256   the matrix pipe: a 256 x 256 x 64 step takes 1.36 us where the panels are in L2, 1.58
