@@ -258,6 +258,8 @@ class UnquantisedMoeLayer:
     def router_logits(self, x):
         """fp32 logits [tokens][experts] of x."""
         experts, hidden = self.cfg.experts, self.cfg.hidden
+        if self.router_weight is None and self.router_weight_16 is None:
+            raise ValueError("the layer has no router: give router_weight or router_weight_16, or call routed()")
         if self.router_weight is None:
             return dense.linear(x, self.router_weight_16).float()
         out = torch.empty(x.shape[0], experts, dtype=torch.float32, device=x.device)

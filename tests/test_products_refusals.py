@@ -127,3 +127,13 @@ def test_calls_of_more_threads_than_a_launch_holds():
     for call in calls:
         with pytest.raises(ValueError, match="more than one launch holds"):
             call()
+
+
+def test_a_layer_without_a_router_takes_given_routing_only():
+    import torch
+    from project_aeon_amd import moe
+    w = torch.zeros(2, 4, 4, dtype=torch.float16)
+    with pytest.raises(ValueError, match="no router"):
+        moe.UnquantisedMoeLayer(w, w, w, 1, 7.0).decode(torch.zeros(1, 4, dtype=torch.float16))
+    with pytest.raises(ValueError, match="fp16 activations"):
+        moe.UnquantisedMoeLayer(w.bfloat16(), w.bfloat16(), w.bfloat16(), 1, 7.0, router_weight=torch.zeros(4, 2))
