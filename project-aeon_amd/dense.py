@@ -47,11 +47,18 @@ def _check(t, name, device, dtype, shape):
     raise ValueError("%s: elements of a row have to follow each other" % name)
 
 
-def _pitch(t):
+def pitch(t):
     """Row pitch of a 2-d tensor: a tensor of one row may carry any stride for it."""
     rows, cols = t.shape
     pitch = t.stride(0)
     return pitch if rows > 1 or pitch > cols else cols
+
+
+def check_rows(t, name, like, cols):
+    """A 2-d tensor of `cols` columns, of the type and on the GPU of `like`."""
+    if t.dim() != 2:
+        raise ValueError("%s has to be a 2-d tensor" % name)
+    _check(t, name, like.get_device(), like.dtype, (t.shape[0], cols))
 
 
 def _ptr(t):
@@ -126,8 +133,8 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
     at, lib = C.addressof(p), capi.lib()
     need = lib.aeon_linear_workspace_bytes(at, tokens)
     ws = _workspace(x, need)
-    _call(device, lib.aeon_linear, at, x.data_ptr(), _pitch(x), tokens, _ptr(residual),
-          0 if residual is None else _pitch(residual), out.data_ptr(), _pitch(out), _ptr(ws), need)
+    _call(device, lib.aeon_linear, at, x.data_ptr(), pitch(x), tokens, _ptr(residual),
+          0 if residual is None else pitch(residual), out.data_ptr(), pitch(out), _ptr(ws), need)
     return out
 
 
@@ -138,6 +145,8 @@ def expert_lists(ids, experts):
     if ids.dim() != 2 or ids.dtype != torch.int32 or not ids.is_cuda or not ids.is_contiguous():
         raise ValueError("ids has to be a contiguous int32 tensor [tokens][slots] on a GPU")
     new = lambda n: torch.empty(n, dtype=torch.int32, device=ids.device)
+    if ids.numel() == 0:
+        return ExpertLists(torch.zeros(experts + 1, dtype=torch.int32, device=ids.device), new(0), new(0))
     lists = ExpertLists(new(experts + 1), new(ids.numel()), new(ids.numel()))
     stream = lambda: C.c_void_p(torch.cuda.current_stream(ids.device).cuda_stream)
     with torch.cuda.device(ids.device):
@@ -167,8 +176,8 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
     positions = x_rows if rows is None else rows.shape[0]
     _lists(device, weight.shape[0], offsets, positions, rows, "rows")
     out = _output(out, x, (positions, p.out_dim))
-    _call(device, capi.lib().aeon_expert_linear, C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), _pitch(x),
-          x_rows, offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), _pitch(out))
+    _call(device, capi.lib().aeon_expert_linear, C.addressof(p), weight.shape[0], _expert_stride(weight, p), x.data_ptr(), pitch(x),
+          x_rows, offsets.data_ptr(), _ptr(rows), positions, out.data_ptr(), pitch(out))
     return out
 
 
@@ -196,7 +205,7 @@ def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None
     at, lib = C.addressof(p), capi.lib()
     need = lib.aeon_expert_combine_workspace_bytes(at, tokens, slots)
     ws = _workspace(h, need)
-    _call(device, lib.aeon_expert_combine, at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), _pitch(h),
+    _call(device, lib.aeon_expert_combine, at, weight.shape[0], _expert_stride(weight, p), h.data_ptr(), pitch(h),
           offsets.data_ptr(), draws.data_ptr(), ids.data_ptr(), weights.data_ptr(), tokens, slots, _ptr(base),
-          0 if base is None else _pitch(base), out.data_ptr(), _pitch(out), _ptr(ws), need)
+          0 if base is None else pitch(base), out.data_ptr(), pitch(out), _ptr(ws), need)
     return out

@@ -249,6 +249,10 @@ class UnquantisedMoeLayer:
             raise ValueError("w1, w3 have to be [experts][intermediate][hidden] and w2 [experts][hidden][intermediate]")
         if router_weight is not None and w1.dtype != torch.float16:
             raise ValueError("the fp32 gate takes fp16 activations; give router_weight_16")
+        for t, name, dtype, shape in ((router_weight, "router_weight", torch.float32, (hidden, experts)),
+                                      (router_bias, "router_bias", torch.float32, (experts,))):
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != w1.device):
+                raise ValueError("%s has to be a contiguous %s tensor of shape %s beside the experts" % (name, dtype, shape))
         self.w1, self.w3, self.w2 = w1, w3, w2
         self.router_weight, self.router_weight_16, self.router_bias = router_weight, router_weight_16, router_bias
         self.dense_shared = dense_shared
@@ -262,23 +266,32 @@ class UnquantisedMoeLayer:
             raise ValueError("the layer has no router: give router_weight or router_weight_16, or call routed()")
         if self.router_weight is None:
             return dense.linear(x, self.router_weight_16).float()
+        dense.check_rows(x, "x", self.w1, hidden)
         out = torch.empty(x.shape[0], experts, dtype=torch.float32, device=x.device)
+        if x.shape[0] == 0:
+            return out
         n = capi.lib().aeon_router_logits_workspace_bytes(x.shape[0], hidden, experts)
         ws = torch.empty(max(n, 4), dtype=torch.uint8, device=x.device)
-        capi.call("aeon_router_logits", capi.vp(x), x.stride(0), capi.vp(self.router_weight), capi.vp(out),
-                  x.shape[0], hidden, experts, capi.vp(ws), C.c_size_t(ws.numel()), stream_ptr())
+        with torch.cuda.device(x.device):
+            capi.call("aeon_router_logits", capi.vp(x), dense.pitch(x), capi.vp(self.router_weight), capi.vp(out),
+                      x.shape[0], hidden, experts, capi.vp(ws), C.c_size_t(ws.numel()), stream_ptr())
         return out
 
     def decode(self, x, out=None, ids=None, weights=None):
         """x [tokens][hidden] -> (out [tokens][hidden], ids int32, weights fp32), MoeLayer.decode's contract."""
         tokens, k = x.shape[0], self.cfg.top_k
+        for t, name, dtype in ((ids, "ids", torch.int32), (weights, "weights", torch.float32)):
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != (tokens, k) or not t.is_contiguous() or t.device != x.device):
+                raise ValueError("%s has to be a contiguous %s tensor [tokens][top_k] beside x" % (name, dtype))
         ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device) if ids is None else ids
         weights = (torch.empty(tokens, k, dtype=torch.float32, device=x.device)
                    if weights is None else weights)
         logits = self.router_logits(x)
-        capi.call("aeon_moe_router", capi.vp(logits), capi.vp(self.router_bias), None, None, capi.vp(weights),
-                  capi.vp(ids), tokens, self.cfg.experts, k, C.c_float(self.cfg.routed_scaling_factor),
-                  self.cfg.renormalize, self.cfg.score_kind, stream_ptr())
+        if tokens > 0:
+            with torch.cuda.device(x.device):
+                capi.call("aeon_moe_router", capi.vp(logits), capi.vp(self.router_bias), None, None, capi.vp(weights),
+                          capi.vp(ids), tokens, self.cfg.experts, k, C.c_float(self.cfg.routed_scaling_factor),
+                          self.cfg.renormalize, self.cfg.score_kind, stream_ptr())
         return self.routed(x, ids, weights, out), ids, weights
 
     def routed(self, x, ids, weights, out=None):

@@ -382,6 +382,35 @@ def test_empty_calls():
     assert dense.expert_combine(none, w, offsets, rows, ids, ids.float()).shape == (0, 16)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_layer_of_no_tokens_and_what_it_refuses(dtype):
+    torch, dense = _setup()
+    from project_aeon_amd import moe
+    dt = _dtype(torch, dtype)
+    E, H, I, k = 4, 128, 64, 2
+    w1, w3, w2 = _normal(torch, (E, I, H), dt, 1), _normal(torch, (E, I, H), dt, 2), _normal(torch, (E, H, I), dt, 3)
+    kw = (dict(router_weight=_normal(torch, (H, E), torch.float32, 4)) if dtype == "f16"
+          else dict(router_weight_16=_normal(torch, (E, H), dt, 4)))
+    layer = moe.UnquantisedMoeLayer(w1, w3, w2, k, LIMIT, **kw)
+    out, ids, weights = layer.decode(torch.empty(0, H, dtype=dt, device="cuda"))
+    assert out.shape == (0, H) and ids.shape == (0, k) and weights.shape == (0, k)
+    x = _normal(torch, (3, H), dt, 5)
+    for bad in (x[:, :64], x.float(), x.reshape(-1), x.cpu(), x.bfloat16() if dtype == "f16" else x.half()):
+        with pytest.raises((ValueError, IndexError)):
+            layer.decode(bad)
+    for given in (dict(ids=torch.empty(3, k, dtype=torch.int64, device="cuda")), dict(ids=torch.empty(2, k, dtype=torch.int32, device="cuda")),
+                  dict(weights=torch.empty(3, k, dtype=dt, device="cuda"))):
+        with pytest.raises(ValueError):
+            layer.decode(x, **given)
+    with pytest.raises(ValueError, match="router_bias"):
+        moe.UnquantisedMoeLayer(w1, w3, w2, k, LIMIT, router_bias=_normal(torch, (E + 1,), torch.float32, 6), **kw)
+    # one row that carries a stride of its own
+    row = _normal(torch, (H, 1), dt, 7).t()
+    assert row.stride() != (H, 1)
+    a, b = layer.decode(row), layer.decode(row.contiguous().clone())
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def test_side_stream_and_two_captured_graphs():
     """The calls on a stream of their own, captured into two graphs that replay in turns between eager
     calls: every replay has the eager result of what its inputs hold then."""
