@@ -253,6 +253,11 @@ class UnquantisedMoeLayer:
                                       (router_bias, "router_bias", torch.float32, (experts,))):
             if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != w1.device):
                 raise ValueError("%s has to be a contiguous %s tensor of shape %s beside the experts" % (name, dtype, shape))
+        gate = router_weight_16  # its rows are the logits of a token: the router reads `experts` of them
+        if gate is not None and (gate.dtype != w1.dtype or tuple(gate.shape) != (experts, hidden) or gate.device != w1.device
+                                 or (hidden > 1 and gate.stride(1) != 1)):
+            raise ValueError("router_weight_16 has to be a %s tensor [experts][hidden] = %s beside the experts, the elements "
+                             "of a row next to each other" % (w1.dtype, (experts, hidden)))
         self.w1, self.w3, self.w2 = w1, w3, w2
         self.router_weight, self.router_weight_16, self.router_bias = router_weight, router_weight_16, router_bias
         self.dense_shared = dense_shared

@@ -137,3 +137,20 @@ def test_a_layer_without_a_router_takes_given_routing_only():
         moe.UnquantisedMoeLayer(w, w, w, 1, 7.0).decode(torch.zeros(1, 4, dtype=torch.float16))
     with pytest.raises(ValueError, match="fp16 activations"):
         moe.UnquantisedMoeLayer(w.bfloat16(), w.bfloat16(), w.bfloat16(), 1, 7.0, router_weight=torch.zeros(4, 2))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_a_layer_checks_the_shape_of_its_16_bit_gate(dtype):
+    """The router is told `experts` logits a token: a gate of another row count would make it read behind
+    them, or at shifted places. Rows wider than the matrix are taken."""
+    import torch
+    from project_aeon_amd import moe
+    dt, E, I, H = getattr(torch, dtype), 8, 4, 16
+    w1, w2 = torch.zeros(E, I, H, dtype=dt), torch.zeros(E, H, I, dtype=dt)
+    other = torch.float16 if dt is torch.bfloat16 else torch.bfloat16
+    for gate in (torch.zeros(E - 1, H, dtype=dt), torch.zeros(E + 1, H, dtype=dt), torch.zeros(E, H - 1, dtype=dt),
+                 torch.zeros(E, H, dtype=other), torch.zeros(E, H), torch.zeros(E * H, dtype=dt),
+                 torch.zeros(H, E, dtype=dt).t(), torch.zeros(E, H, dtype=dt, device="meta")):
+        with pytest.raises(ValueError, match="router_weight_16"):
+            moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0, router_weight_16=gate)
+    moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0, router_weight_16=torch.zeros(E, H + 3, dtype=dt)[:, :H])
