@@ -300,9 +300,15 @@ class UnquantisedMoeLayer:
         return self.routed(x, ids, weights, out), ids, weights
 
     def routed(self, x, ids, weights, out=None):
-        """The expert part for given routing. Without an always-on expert the routed sum is added to what
-        `out` holds (an `out` allocated here starts from zero), as MoeLayer.routed does."""
+        """The expert part for given routing, ids int32 and weights fp32 [tokens][slots]. Without an always-on
+        expert the routed sum is added to what `out` holds (an `out` allocated here starts from zero), as
+        MoeLayer.routed does."""
         limit = self.cfg.swiglu_limit
+        if ids.dim() != 2 or ids.shape[0] != x.shape[0]:
+            raise ValueError("ids has to be [tokens][slots] of x: shape %s for %d tokens" % (tuple(ids.shape), x.shape[0]))
+        if weights.shape != ids.shape:
+            raise ValueError("weights has to be [tokens][slots] as ids is: shape %s, not %s"
+                             % (tuple(weights.shape), tuple(ids.shape)))
         base = out
         if self.dense_shared is not None:
             w1, w3, w2 = self.dense_shared

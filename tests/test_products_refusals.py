@@ -154,3 +154,21 @@ def test_a_layer_checks_the_shape_of_its_16_bit_gate(dtype):
         with pytest.raises(ValueError, match="router_weight_16"):
             moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0, router_weight_16=gate)
     moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0, router_weight_16=torch.zeros(E, H + 3, dtype=dt)[:, :H])
+
+
+def test_a_layer_refuses_a_routing_of_other_tokens():
+    """ids and weights are [tokens][slots] of the given x: rows of ids beyond x would be sums over hidden rows that
+    no product wrote, fewer would leave tokens out."""
+    import torch
+    from project_aeon_amd import moe
+    E, I, H = 4, 4, 16
+    w1, w2 = torch.zeros(E, I, H, dtype=torch.float16), torch.zeros(E, H, I, dtype=torch.float16)
+    layer = moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0)
+    x = torch.zeros(3, H, dtype=torch.float16)
+    ids, weights = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2)
+    for bad in (ids[:2], torch.zeros(5, 2, dtype=torch.int32), ids.reshape(-1), ids[:0]):
+        with pytest.raises(ValueError, match="ids has to be .*3 tokens"):
+            layer.routed(x, bad, torch.zeros(bad.shape))
+    for bad in (weights[:2], weights[:, :1], torch.zeros(5, 2)):
+        with pytest.raises(ValueError, match="weights has to be"):
+            layer.routed(x, ids, bad)
