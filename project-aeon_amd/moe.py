@@ -272,6 +272,8 @@ class UnquantisedMoeLayer:
         if self.router_weight is None:
             return dense.linear(x, self.router_weight_16).float()
         dense.check_rows(x, "x", self.w1, hidden)
+        if dense.pitch(x) >= 1 << 31:
+            raise ValueError("x has a row pitch of %d elements: the fp32 gate takes fewer than 2^31" % dense.pitch(x))
         out = torch.empty(x.shape[0], experts, dtype=torch.float32, device=x.device)
         if x.shape[0] == 0:
             return out

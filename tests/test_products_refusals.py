@@ -172,3 +172,16 @@ def test_a_layer_refuses_a_routing_of_other_tokens():
     for bad in (weights[:2], weights[:, :1], torch.zeros(5, 2)):
         with pytest.raises(ValueError, match="weights has to be"):
             layer.routed(x, ids, bad)
+
+
+def test_a_layer_refuses_rows_too_far_apart_for_the_fp32_gate():
+    """aeon_router_logits takes the row pitch as an int; 2^32 + 16 elements would pass as 16."""
+    import torch
+    from project_aeon_amd import moe
+    E, I, H = 4, 4, 16
+    w1 = torch.zeros(E, I, H, dtype=torch.float16, device="meta")
+    w2 = torch.zeros(E, H, I, dtype=torch.float16, device="meta")
+    layer = moe.UnquantisedMoeLayer(w1, w1, w2, 2, 7.0, router_weight=torch.zeros(H, E, device="meta"))
+    far = torch.empty((1 << 33), dtype=torch.float16, device="meta").as_strided((2, H), ((1 << 32) + H, 1))
+    with pytest.raises(ValueError, match="pitch"):
+        layer.router_logits(far)
