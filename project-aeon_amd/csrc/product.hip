@@ -1195,8 +1195,10 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
         best_us = 1.4 + n / 8 * ((tokens + kFewMax - 1) / kFewMax) * each;
     }
     for (const TileCost& t : kTileCosts) {
-        // tiles that would stay half empty, or be far too many
-        if (t.positions > 64 ? t.positions > 2L * tokens : t.rows < 64 && (t.positions < 64 ? tokens > 128 : tokens > 512)) continue;
+        // tiles that would stay half empty, or be far too many. A window of at most 128 positions makes a 256 x 256
+        // step no shorter where the weights come from memory. Measured, us in it / in 128 x 128, 128 tokens: 4096 -> 14336:
+        // 68 / 46, 7168 -> 28672: 128 / 87; 7168 -> 65536 is the exception, 178 / 193.
+        if (t.positions > 64 ? t.positions >= 2L * tokens : t.rows < 64 && (t.positions < 64 ? tokens > 128 : tokens > 512)) continue;
         const double tiles = static_cast<double>((tokens + t.positions - 1) / t.positions) *
                              ((static_cast<long>(n) + t.rows - 1) / t.rows);
         for (int splits : {1, 2, 3, 4, 6, 8}) {
@@ -1209,10 +1211,9 @@ static ProductPlan plan_linear(const aeon_projection& w, int tokens) {
             if (last > 0) {
                 double step = last <= 256 ? t.step_alone : t.step_shared;
                 // a last round of the waves that take turns is cut into halves of 0.55 of a tile's products
-                if (t.tile == kTile256 && last <= 128 && splits == 1 && tokens > 128) step *= 0.55;
+                if (t.tile == kTile256 && last <= 128 && splits == 1) step *= 0.55;
                 us += each * step + t.fixed;
             }
-            if (t.tile == kTile256 && tokens <= 128) us *= 0.55;
             if (us < stream) us = stream;
             if (splits > 1) us += 0.7 + 8.0 * splits * tokens * n / 14.5e6;
             if (best_us == 0.0 || us < best_us) {
