@@ -304,22 +304,21 @@ class UnquantisedMoeLayer:
     def routed(self, x, ids, weights, out=None):
         """The expert part for given routing, ids int32 and weights fp32 [tokens][slots]. Without an always-on
         expert the routed sum is added to what `out` holds (an `out` allocated here starts from zero), as
-        MoeLayer.routed does."""
+        MoeLayer.routed does. `out` may be x."""
         limit = self.cfg.swiglu_limit
         if ids.dim() != 2 or ids.shape[0] != x.shape[0]:
             raise ValueError("ids has to be [tokens][slots] of x: shape %s for %d tokens" % (tuple(ids.shape), x.shape[0]))
         if weights.shape != ids.shape:
             raise ValueError("weights has to be [tokens][slots] as ids is: shape %s, not %s"
                              % (tuple(weights.shape), tuple(ids.shape)))
-        base = out
-        if self.dense_shared is not None:
-            w1, w3, w2 = self.dense_shared
-            h = dense.linear(x, w1, weight_up=w3, activation="swiglu", swiglu_limit=limit)
-            base = out = dense.linear(h, w2, out=out)
+        # x is read to the end before `out` is written: the two may be one tensor
         lists = dense.expert_lists(ids, self.cfg.experts)
         h = dense.expert_linear(x, self.w1, lists.offsets, lists.rows, weight_up=self.w3, activation="swiglu",
                                 swiglu_limit=limit)
-        return dense.expert_combine(h, self.w2, lists.offsets, lists.draws, ids, weights, base=base, out=out)
+        if self.dense_shared is not None:
+            w1, w3, w2 = self.dense_shared
+            out = dense.linear(dense.linear(x, w1, weight_up=w3, activation="swiglu", swiglu_limit=limit), w2, out=out)
+        return dense.expert_combine(h, self.w2, lists.offsets, lists.draws, ids, weights, base=out, out=out)
 
 
 class HyperConnection:
