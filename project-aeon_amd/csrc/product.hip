@@ -884,15 +884,43 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(const Produ
 // 8 slots, 2048 -> 7168: 41.8 / 48.6 and 108 / 109; 8 tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.2 / 10.3; 12 tokens
 // (50 MB): 13.5 / 10.3; 4 tokens of 6 slots, 512 -> 2048 (50 MB): 13.3 / 16.5, 6 tokens (75 MB): 19.6 / 18.7. The host
 // spends 4 us less on it.
+// The weight meets a slot's whole product, as in two launches: a weighed part may be infinite, or NaN beside an
+// infinite weight, where the product is neither.
 constexpr int kDirectDraws = 64;
 constexpr int kDirectTokens = 3;
 constexpr double kDirectBytes = 40e6;  // rows streamed, above which more tokens go through memory
+// Sums over the lanes of eight values a lane: of value lane % 8. Three exchanges halve the values a lane holds (with
+// lane ^ 7, ^ 2 and ^ 1, which reach all eight), three steps add what is left over lanes 8, 16 and 32 apart. All of it in
+// the vector pipe, seven moves and three steps: a butterfly through LDS for each value is 48 round trips.
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float sum_by_row(const float (&v)[8], int lane) {
+    constexpr int kXor7 = 0x141, kXor2 = 0x4E, kXor1 = 0xB1, kXor8 = 0x128;  // row_half_mirror, quad_perm twice, row_ror:8
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = (lane & 4 ? v[i + 4] : v[i]) + from_lane<kXor7>(lane & 4 ? v[i] : v[i + 4]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = (lane & 2 ? a[i + 2] : a[i]) + from_lane<kXor2>(lane & 2 ? a[i] : a[i + 2]);
+    float c = (lane & 1 ? b[1] : b[0]) + from_lane<kXor1>(lane & 1 ? b[0] : b[1]);
+    c += from_lane<kXor8>(c);
+    // the rows of 16 lanes of a pair, then the halves of the wave, change places: the two results add up to the sum
+    auto joined = [](auto pair) {
+        const uint32_t one = pair[0], two = pair[1];
+        return __builtin_bit_cast(float, one) + __builtin_bit_cast(float, two);
+    };
+    uint32_t bits = __builtin_bit_cast(uint32_t, c);
+    bits = __builtin_bit_cast(uint32_t, joined(__builtin_amdgcn_permlane16_swap(bits, bits, false, false)));
+    return joined(__builtin_amdgcn_permlane32_swap(bits, bits, false, false));
+}
+
 template <class T, int ROWS>
 __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const ProductArgs a, const int32_t* ids, int slots,
                                                                        const uint16_t* base, long base_stride,
                                                                        uint16_t* out, long out_stride) {
     typedef u32x4_t __attribute__((aligned(2))) loose_t;
-    __shared__ float sums[ROWS][kFewWaves];
+    __shared__ float sums[kDirectDraws][ROWS][kFewWaves];  // by slot
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int token = blockIdx.y;
@@ -925,6 +953,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
     struct Load {
         u32x4_t w[ROWS], x;
         int slot, c;
+        bool last;  // of the slot's chunks in this wave
     } load[2];
     auto issue = [&](Load& l) __attribute__((always_inline)) {
         const int expert = __builtin_amdgcn_readlane(id, slot);
@@ -933,6 +962,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
         const int from = c < a.k - 8 ? c : a.k - 8;
         l.slot = slot;
         l.c = c;
+        l.last = at + kFewWaves * 512 >= a.k;
         const AEON_GLOBAL uint16_t* w = as_global<uint16_t>(a.w[0]) + expert * a.expert_stride;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -941,9 +971,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
         }
         l.x = *reinterpret_cast<const AEON_GLOBAL loose_t*>(as_global<uint16_t>(a.x) + p * a.x_stride + from);
     };
-    float total[ROWS] = {};
+    float dot[ROWS] = {};
     auto use = [&](Load& l) __attribute__((always_inline)) {
-        const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), l.slot));
         u32x4_t keep;  // the values before column c are the lane before's (row_dots)
         const int over = l.c < a.k - 8 ? 0 : l.c - (a.k - 8);
 #pragma unroll
@@ -952,12 +981,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
         widen8<T>(l.x & keep, x);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            float w[8], dot = 0.0f;
+            float w[8];
             widen8<T>(l.w[r] & keep, w);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) dot = fmaf(w[q], x[q], dot);
-            total[r] = fmaf(scale, dot, total[r]);
+            for (int q = 0; q < 8; ++q) dot[r] = fmaf(w[q], x[q], dot[r]);
         }
+        if (!l.last) return;
+        const float sum = sum_by_row(dot, lane);
+        if (lane < ROWS) sums[l.slot][lane][wave] = sum;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) dot[r] = 0.0f;
     };
     const uint64_t all_slots = slots_left;
     bool more = next();
@@ -971,28 +1004,25 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
         if (more) issue(load[0]);
         use(load[1]);
     }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        const float v = wave_xor_sum(total[r], 63);
-        if (lane == 0) sums[r][wave] = v;
-    }
     __syncthreads();
     if (wave != 0) return;
+    const int waves = (a.k + 511) / 512 < kFewWaves ? (a.k + 511) / 512 : kFewWaves;  // that had a chunk
     const int o = n0 + lane;
     const bool live = lane < ROWS && o < a.n;
     float y = 0.0f;
-    if (live) y = ((sums[lane][0] + sums[lane][1]) + sums[lane][2]) + sums[lane][3];
-    if (a.bias[0] != nullptr) {
-        for (uint64_t left = all_slots; left != 0; left &= left - 1) {
-            const int s = __builtin_ctzll(left);
-            const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), s));
-            const int expert = __builtin_amdgcn_readlane(id, s);
-            if (live) y = fmaf(scale, T::widen(a.bias[0][static_cast<size_t>(expert) * a.n + o]), y);
+    if (live && base != nullptr) y = T::widen(base[token * base_stride + o]);
+    for (uint64_t left = all_slots; left != 0; left &= left - 1) {
+        const int s = __builtin_ctzll(left);
+        const float scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), s));
+        const int expert = __builtin_amdgcn_readlane(id, s);
+        if (live) {
+            float v = sums[s][lane][0];
+            for (int i = 1; i < waves; ++i) v += sums[s][lane][i];
+            if (a.bias[0] != nullptr) v += T::widen(a.bias[0][static_cast<size_t>(expert) * a.n + o]);
+            y += v * scale;
         }
     }
-    if (!live) return;
-    if (base != nullptr) y += T::widen(base[token * base_stride + o]);
-    out[token * out_stride + o] = T::round(y);
+    if (live) out[token * out_stride + o] = T::round(y);
 }
 
 // Joins the shares of K of a dense product, in share order, and applies the epilogue. Four outputs

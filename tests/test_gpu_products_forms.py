@@ -14,10 +14,25 @@ def _setup():
     return torch, dense, moe
 
 
+def _whole(torch, shape, dtype, seed, span=2):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randint(-span, span + 1, shape, generator=g, device="cuda").to(dtype)
+
+
 def _normal(torch, shape, dtype, seed, std=1.0):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
     return (torch.randn(shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def _mm64(x, w):
+    return x.double() @ w.double().t().contiguous()
+
+
+def _same(torch, got, want):
+    """Equal, NaN where NaN is due and nowhere else."""
+    return torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
 
 
 @pytest.mark.parametrize("shared", [False, True])
@@ -37,3 +52,63 @@ def test_a_layer_may_write_its_output_over_its_input(tokens, shared):
     got = layer.decode(x, out=x)
     assert got[0].data_ptr() == x.data_ptr()
     assert torch.equal(got[0], want) and torch.equal(got[1], ids) and torch.equal(got[2], weights)
+
+
+def _spread(torch, tokens, slots, experts):
+    """ids that put the draws of a token on different experts, and their lists."""
+    ids = (torch.arange(tokens * slots, device="cuda") * 3 % experts).to(torch.int32).view(tokens, slots)
+    return ids
+
+
+# draws and matrices on both sides of what one launch takes, K with and without a last partial chunk of 512, K of
+# one lane, K of more chunks than waves
+COMBINE_SHAPES = [(1, 8, 16, 1030, 48), (1, 8, 16, 2048, 520), (3, 4, 16, 72, 130), (2, 1, 5, 8, 9), (8, 2, 7, 4104, 24),
+                  (1, 3, 5, 7, 16), (20, 4, 16, 1030, 48), (40, 2, 16, 520, 130)]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("tokens,slots,experts,k,n", COMBINE_SHAPES)
+def test_combine_takes_weights_that_are_not_finite(tokens, slots, experts, k, n, dtype):
+    """weight * (W_e h + b): an infinite weight gives the product's sign, NaN gives NaN, whatever way the product
+    was summed. Whole numbers, so that the products are exact and the 64-bit formula has the same infinities."""
+    torch, dense, moe = _setup()
+    dt = getattr(torch, dtype)
+    ids = _spread(torch, tokens, slots, experts)
+    lists = dense.expert_lists(ids, experts)
+    draws = lists.draws.long()
+    h, w = _whole(torch, (tokens * slots, k), dt, 1), _whole(torch, (experts, n, k), dt, 2)
+    b = _whole(torch, (experts, n), dt, 3, 9)
+    by_draw = torch.empty(tokens * slots, n, dtype=torch.float64, device="cuda")
+    flat = ids.reshape(-1).long()
+    for p, d in enumerate(draws.tolist()):
+        by_draw[d] = _mm64(h[p:p + 1], w[flat[d]])[0] + b[flat[d]].double()
+    by_draw = by_draw.view(tokens, slots, n)
+    inf, nan = float("inf"), float("nan")
+    for i, special in enumerate((inf, -inf, nan, 0.0)):
+        weights = _whole(torch, (tokens, slots), torch.float32, 5)
+        weights[i % tokens, i % slots] = special
+        print("combine", tokens, slots, experts, k, n, dtype, special, flush=True)
+        want = (by_draw * weights.double().unsqueeze(2)).sum(dim=1)
+        got = dense.expert_combine(h, w, lists.offsets, lists.draws, ids, weights, bias=b)
+        assert _same(torch, got, want.to(dt))
+    weights = torch.ones(tokens, slots, device="cuda")
+    weights[0, 0], weights[0, slots - 1] = inf, -inf  # NaN where the products have one sign, infinity elsewhere
+    want = (by_draw * weights.double().unsqueeze(2)).sum(dim=1)
+    assert _same(torch, dense.expert_combine(h, w, lists.offsets, lists.draws, ids, weights, bias=b), want.to(dt))
+
+
+@pytest.mark.parametrize("tokens", [1, 80])   # in one launch, and in two
+@pytest.mark.parametrize("k", [512, 1024, 4096])
+def test_combine_weighs_the_product_and_not_its_parts(tokens, k):
+    """Parts of 2^11 that cancel to 2^4, times a weight of 2^118: the result is 2^122, though a weighed part would
+    be beyond fp32."""
+    torch, dense, moe = _setup()
+    dt, n = torch.bfloat16, 40
+    h = torch.full((tokens, k), 16.0, dtype=dt, device="cuda")
+    h[:, torch.arange(k, device="cuda") // 8 % 2 == 1] = -16.0
+    h[:, 0] = 17.0
+    w = torch.full((2, n, k), 16.0, dtype=dt, device="cuda")
+    ids = torch.ones(tokens, 1, dtype=torch.int32, device="cuda")
+    lists = dense.expert_lists(ids, 2)
+    out = dense.expert_combine(h, w, lists.offsets, lists.draws, ids, torch.full((tokens, 1), 2.0 ** 118, device="cuda"))
+    assert bool((out.double() == 2.0 ** 122).all())
