@@ -413,15 +413,19 @@ class LayerStack:
     weightless norm = the FFN norm the reference's layer body applies to the layer input
     (layer/v4_layer_body_attention.hpp:113-115). `fused` runs the reduce, the post-mix and the
     next layer's pre-combine in the expert step's last launch instead of three launches of
-    their own; same bits."""
+    their own; same bits. Layers of unquantised experts have no such launch: with one of them among
+    `layers` the stack runs the three. They have to be fp16, as the residual streams and the mixes are."""
 
     def __init__(self, layers, mixes, norm_weights=None, fused=True, rms_eps=1e-6):
         assert len(layers) == len(mixes)
         assert norm_weights is None or len(norm_weights) == len(layers)
+        for layer in layers:
+            if isinstance(layer, UnquantisedMoeLayer) and layer.w1.dtype != torch.float16:
+                raise ValueError("the stack's residual streams are fp16: a layer of %s experts does not run in it" % layer.w1.dtype)
         self.layers = layers
         self.mixes = mixes
         self.norm_weights = norm_weights
-        self.fused = fused
+        self.fused = fused and all(hasattr(layer, "decode_hc_post") for layer in layers)
         self.rms_eps = rms_eps
 
     def _norm(self, l, x, out):

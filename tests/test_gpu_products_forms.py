@@ -1,5 +1,6 @@
 """GPU parity of the unquantised layer and its products where a call is unlike the usual one: outputs on the input,
 routing weights that are not finite or far larger than a value, gates whose logits need more than 16 bits."""
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +113,21 @@ def test_combine_weighs_the_product_and_not_its_parts(tokens, k):
     lists = dense.expert_lists(ids, 2)
     out = dense.expert_combine(h, w, lists.offsets, lists.draws, ids, torch.full((tokens, 1), 2.0 ** 118, device="cuda"))
     assert bool((out.double() == 2.0 ** 122).all())
+
+
+def test_a_stack_of_unquantised_layers_as_it_defaults():
+    """LayerStack(layers, mixes) with nothing else said: the bits of the stack without the fused tail."""
+    torch, dense, moe = _setup()
+    from project_aeon_amd import synth
+    H, I, E, k, tokens, dt = 256, 128, 16, 2, 9, torch.float16
+    layers, mixes = [], []
+    for l in range(2):
+        w1, w3 = (_normal(torch, (E, I, H), dt, 10 * l + s, H ** -0.5) for s in (2, 3))
+        w2 = _normal(torch, (E, H, I), dt, 10 * l + 4, I ** -0.5)
+        gate = torch.from_numpy(synth.router_weight(l, H, E)).cuda()
+        layers.append(moe.UnquantisedMoeLayer(w1, w3, w2, k, LIMIT, router_weight=gate))
+        mixes.append(moe.HyperConnection(np.random.default_rng(l).normal(size=24)))
+    residual = _normal(torch, (4, tokens, H), dt, 1)
+    got = moe.LayerStack(layers, mixes).step(residual.clone())
+    want = moe.LayerStack(layers, mixes, fused=False).step(residual.clone())
+    assert torch.equal(got, want) and bool(got.isfinite().all())

@@ -185,3 +185,18 @@ def test_a_layer_refuses_rows_too_far_apart_for_the_fp32_gate():
     far = torch.empty((1 << 33), dtype=torch.float16, device="meta").as_strided((2, H), ((1 << 32) + H, 1))
     with pytest.raises(ValueError, match="pitch"):
         layer.router_logits(far)
+
+
+def test_a_stack_takes_unquantised_layers_of_fp16_only():
+    """The residual streams and their mixes are fp16. Layers without the fused tail run in the three launches."""
+    import torch
+    from project_aeon_amd import moe
+
+    def layer(dtype):
+        w1, w2 = torch.zeros(2, 4, 8, dtype=dtype), torch.zeros(2, 8, 4, dtype=dtype)
+        return moe.UnquantisedMoeLayer(w1, w1, w2, 1, 7.0)
+
+    assert moe.LayerStack([layer(torch.float16)], [None]).fused is False
+    assert moe.LayerStack([], []).fused is True
+    with pytest.raises(ValueError, match="fp16"):
+        moe.LayerStack([layer(torch.float16), layer(torch.bfloat16)], [None, None])
