@@ -237,6 +237,16 @@ int aeon_router_logits_f16(const void* d_x, int x_stride, const void* d_gate_wei
                            void* d_logits_half, float* d_logits, int tokens, int hidden,
                            int experts, void* stream);
 
+/* The logits of a bf16 gate and bf16 activations: logits[t][e] = sum_h x[t][h] * w[e][h], fp32 sums in
+ * a fixed order that are not rounded to the 8 bits of bf16 (the experts a token goes to are chosen
+ * by their differences). d_gate_weight [experts][hidden], row pitch gate_stride elements; any
+ * size and pitch. The workspace (16-byte boundary, 0 bytes where nothing is cut) holds shares of
+ * the sums over hidden. */
+size_t aeon_router_logits_bf16_workspace_bytes(int tokens, int hidden, int experts);
+int aeon_router_logits_bf16(const void* d_x, long x_stride, const void* d_gate_weight, long gate_stride,
+                            float* d_logits, int tokens, int hidden, int experts, void* d_workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* gemv_fp16_vec8_kernel launch, src/platform/ops/gemv.hpp:72-110, for `tokens` rows at once:
  * y[t][o] = half(sum_i x[t][i] * w[o][i]), w fp16 [out_dim][in_dim] row-major, fp32 accumulate.
  * in_dim % 128 == 0, out_dim % 16 == 0, x_stride % 8 == 0, y_stride % 4 == 0. */

@@ -75,6 +75,8 @@ def lib():
         for name, result, args in (
                 ("aeon_linear_workspace_bytes", C.c_size_t, (p, i)),
                 ("aeon_linear", i, (p, p, n, i, p, n, p, n, p, C.c_size_t, p)),
+                ("aeon_router_logits_bf16_workspace_bytes", C.c_size_t, (i, i, i)),
+                ("aeon_router_logits_bf16", i, (p, n, p, n, p, i, i, i, p, C.c_size_t, p)),
                 ("aeon_expert_linear", i, (p, i, n, p, n, i, p, p, i, p, n, p)),
                 ("aeon_expert_combine_workspace_bytes", C.c_size_t, (p, i, i)),
                 ("aeon_expert_combine", i, (p, i, n, p, n, p, p, p, p, i, i, p, n, p, n, p, C.c_size_t, p))):

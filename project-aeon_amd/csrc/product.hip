@@ -855,6 +855,10 @@ __device__ __forceinline__ void few_body(const ProductArgs& a, const ProductTile
         if (draw >= 0 && draw < a.draw_count) a.wide[static_cast<size_t>(draw) * a.n + o] = g * a.draw_weights[draw];
         return;
     }
+    if (a.mode == kProductPartial) {
+        a.wide[static_cast<size_t>(p) * a.n + o] = g;
+        return;
+    }
     if (a.rows != nullptr) {
         const int row = a.rows[p];
         if (row < 0 || row >= a.x_rows) return;
@@ -1025,10 +1029,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const Pro
     if (live) out[token * out_stride + o] = T::round(y);
 }
 
-// Joins the shares of K of a dense product, in share order, and applies the epilogue. Four outputs
-// a thread.
+// Joins the shares of K of a dense product, in share order, and applies the epilogue, or leaves the sums in `sums`
+// as they are (a product without epilogue). Four outputs a thread.
 template <class T>
-__global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, int splits) {
+__global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, int splits, float* sums) {
     const int groups = (a.n + 3) / 4;
     const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
     if (at >= static_cast<long>(a.positions) * groups) return;
@@ -1041,6 +1045,10 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a, 
         const float* src = a.wide + static_cast<size_t>(s) * mats * share + static_cast<size_t>(p) * a.n + o;
         sum[0] += load_wide(src, o, a.n);
         if (a.pair) sum[1] += load_wide(src + share, o, a.n);
+    }
+    if (sums != nullptr) {
+        store_wide(sums + static_cast<size_t>(p) * a.n + o, sum[0], o, a.n);
+        return;
     }
     float v[4], u[4];
     if (a.bias[0] != nullptr) sum[0] += load_narrow<T>(a.bias[0] + o, o, a.n);
@@ -1345,6 +1353,20 @@ static size_t linear_workspace(const aeon_projection& w, int tokens, const Produ
     return static_cast<size_t>(p.splits) * (w.activation == AEON_ACT_SWIGLU ? 2 : 1) * tokens * w.out_dim * sizeof(float);
 }
 
+// Shares of K into a.wide, and the launch that joins more than one of them: by the epilogue, or into `sums`.
+static int launch_shares(int dtype, const ProductPlan& plan, ProductArgs& a, float* sums, hipStream_t stream) {
+    a.mode = kProductPartial;
+    a.split_steps = plan.split_steps;
+    if (int rc = launch_product(dtype, plan.tile, a, plan.splits, stream)) return rc;
+    if (plan.splits == 1) return AEON_OK;
+    const long threads = static_cast<long>(a.positions) * ((a.n + 3) / 4);
+    const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+    if (dtype == AEON_DTYPE_F16) product_join_kernel<F16><<<blocks, 256, 0, stream>>>(a, plan.splits, sums);
+    else product_join_kernel<BF16><<<blocks, 256, 0, stream>>>(a, plan.splits, sums);
+    AEON_LAUNCH_CHECK();
+    return AEON_OK;
+}
+
 }  // namespace aeon355
 
 using namespace aeon355;
@@ -1385,16 +1407,45 @@ extern "C" int aeon_linear(const aeon_projection* projection, const void* d_x, l
     a.y = static_cast<uint16_t*>(d_y);
     a.y_stride = y_stride;
     if (plan.splits == 1) return launch_product(w.dtype, plan.tile, a, 1, as_stream(stream));
-    a.mode = kProductPartial;
     a.wide = static_cast<float*>(d_workspace);
-    a.split_steps = plan.split_steps;
-    if (int rc = launch_product(w.dtype, plan.tile, a, plan.splits, as_stream(stream))) return rc;
-    const long threads = static_cast<long>(tokens) * ((w.out_dim + 3) / 4);
-    const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-    if (w.dtype == AEON_DTYPE_F16) product_join_kernel<F16><<<blocks, 256, 0, as_stream(stream)>>>(a, plan.splits);
-    else product_join_kernel<BF16><<<blocks, 256, 0, as_stream(stream)>>>(a, plan.splits);
-    AEON_LAUNCH_CHECK();
-    return AEON_OK;
+    return launch_shares(w.dtype, plan, a, nullptr, as_stream(stream));
+}
+
+// The gate as a projection without bias or activation.
+static aeon_projection gate_projection(const void* d_gate, long gate_stride, int hidden, int experts) {
+    return aeon_projection{AEON_DTYPE_BF16, hidden, experts, AEON_ACT_NONE, d_gate, nullptr, gate_stride, nullptr, nullptr, 0.0f};
+}
+
+extern "C" size_t aeon_router_logits_bf16_workspace_bytes(int tokens, int hidden, int experts) {
+    if (tokens <= 0 || tokens > kMostPositions || hidden <= 0 || experts <= 0) return 0;
+    const aeon_projection w = gate_projection(nullptr, hidden, hidden, experts);
+    return linear_workspace(w, tokens, plan_linear(w, tokens));
+}
+
+extern "C" int aeon_router_logits_bf16(const void* d_x, long x_stride, const void* d_gate_weight, long gate_stride, float* d_logits,
+                                       int tokens, int hidden, int experts, void* d_workspace, size_t workspace_bytes,
+                                       void* stream) {
+    const char* who = "aeon_router_logits_bf16";
+    const aeon_projection w = gate_projection(d_gate_weight, gate_stride, hidden, experts);
+    if (int rc = check_projection(&w, who)) return rc;
+    AEON_REQUIRE(tokens >= 0 && tokens <= kMostPositions, AEON_ERR_INVALID_ARGUMENT, "%s: token count out of range (%d)", who, tokens);
+    if (tokens == 0) return AEON_OK;
+    AEON_REQUIRE(d_x && d_logits, AEON_ERR_INVALID_ARGUMENT, "%s: null buffer", who);
+    AEON_REQUIRE(on_boundary(d_x, 2) && on_boundary(d_logits, 4), AEON_ERR_INVALID_ARGUMENT,
+                 "%s: an operand starts off its element's boundary", who);
+    AEON_REQUIRE(x_stride >= hidden, AEON_ERR_INVALID_ARGUMENT, "%s: bad row pitch (x %ld)", who, x_stride);
+    AEON_REQUIRE(d_logits != d_x && d_logits != d_gate_weight, AEON_ERR_INVALID_ARGUMENT,
+                 "%s: the output must not alias the activations or the weights", who);
+    const ProductPlan plan = plan_linear(w, tokens);
+    if (int rc = check_workspace(d_workspace, workspace_bytes, linear_workspace(w, tokens, plan), who)) return rc;
+    ProductArgs a = projection_args(w);
+    a.x = static_cast<const uint16_t*>(d_x);
+    a.x_stride = x_stride;
+    a.x_rows = tokens;
+    a.positions = tokens;
+    // one share of K is the whole sum: it goes where a share would
+    a.wide = plan.splits == 1 ? d_logits : static_cast<float*>(d_workspace);
+    return launch_shares(w.dtype, plan, a, d_logits, as_stream(stream));
 }
 
 extern "C" int aeon_expert_linear(const aeon_projection* projection, int experts, long expert_stride,

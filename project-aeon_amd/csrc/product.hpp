@@ -9,7 +9,7 @@ namespace aeon355 {
 enum ProductMode : int {
     kProductRows = 0,     // y[position][n] in the operands' type, after activation and residual
     kProductDraws = 1,    // contrib[draw][n] fp32 = weight[draw] * (W h + b)
-    kProductPartial = 2,  // partial[split][matrix][token][n] fp32, joined by a second launch
+    kProductPartial = 2,  // partial[split][matrix][token][n] fp32, without epilogue; several are joined by a second launch
 };
 
 struct ProductArgs {

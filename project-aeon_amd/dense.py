@@ -138,6 +138,23 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
     return out
 
 
+def router_logits(x, gate):
+    """fp32 [tokens][experts]: the sums x @ gate.T of a bf16 gate [experts][hidden], unrounded
+    (aeon_router_logits_bf16)."""
+    if gate.dim() != 2 or gate.dtype is not torch.bfloat16 or not gate.is_cuda:
+        raise ValueError("gate has to be a 2-d bf16 tensor on a GPU")
+    experts, hidden = gate.shape
+    check_rows(gate, "gate", gate, hidden)
+    check_rows(x, "x", gate, hidden)
+    device, tokens, lib = gate.get_device(), x.shape[0], capi.lib()
+    out = x.new_empty((tokens, experts), dtype=torch.float32)
+    need = lib.aeon_router_logits_bf16_workspace_bytes(tokens, hidden, experts)
+    ws = _workspace(x, need)
+    _call(device, lib.aeon_router_logits_bf16, x.data_ptr(), pitch(x), gate.data_ptr(), pitch(gate), out.data_ptr(), tokens,
+          hidden, experts, _ptr(ws), need)
+    return out
+
+
 def expert_lists(ids, experts):
     """The ragged lists of a routing, ids int32 [tokens][slots] (aeon_expert_permutation): expert e holds
     positions offsets[e] .. offsets[e+1]-1, its draws (token * slots + slot) ascending; ids outside

@@ -239,8 +239,10 @@ class UnquantisedMoeLayer:
     [experts][hidden][intermediate] of one type, fp16 or bf16, which is the activations' too. The same
     router, permutation and roundings (hidden rows in that type, contributions fp32, slots in order), for
     one token as for a prefill chunk. `dense_shared`: (w1, w3, w2) of an always-on expert, its output
-    the value the routed sum starts from. The router is MoeLayer's for fp16 activations; for bf16 the gate
-    is router_weight_16, bf16 [experts][hidden], with logits rounded to bf16."""
+    the value the routed sum starts from. The router is MoeLayer's for fp16 activations (an fp16 gate's
+    logits are rounded to fp16, as the fp16 checkpoint's own path does); for bf16 the gate is
+    router_weight_16, bf16 [experts][hidden], with logits in fp32: rounded to 8 bits they would send about
+    one token in 25 to another set of experts (top-8 of 256 normal logits)."""
 
     def __init__(self, w1, w3, w2, top_k, swiglu_limit, router_weight=None, router_bias=None, score_kind=1,
                  routed_scaling_factor=1.0, renormalize=True, router_weight_16=None, dense_shared=None):
@@ -269,6 +271,8 @@ class UnquantisedMoeLayer:
         experts, hidden = self.cfg.experts, self.cfg.hidden
         if self.router_weight is None and self.router_weight_16 is None:
             raise ValueError("the layer has no router: give router_weight or router_weight_16, or call routed()")
+        if self.router_weight is None and self.router_weight_16.dtype == torch.bfloat16:
+            return dense.router_logits(x, self.router_weight_16)
         if self.router_weight is None:
             return dense.linear(x, self.router_weight_16).float()
         dense.check_rows(x, "x", self.w1, hidden)

@@ -131,3 +131,28 @@ def test_a_stack_of_unquantised_layers_as_it_defaults():
     got = moe.LayerStack(layers, mixes).step(residual.clone())
     want = moe.LayerStack(layers, mixes, fused=False).step(residual.clone())
     assert torch.equal(got, want) and bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("tokens,hidden,experts", [(1, 4096, 256), (1, 100, 7), (3, 512, 24), (20, 7168, 256), (33, 520, 40),
+                                                   (64, 4100, 80), (300, 520, 130), (9, 2049, 16), (40, 4101, 80), (5, 7, 4)])
+def test_logits_of_a_bf16_gate_are_not_rounded(tokens, hidden, experts):
+    """Whole numbers whose sums need more than the 8 bits of bf16: exact in fp32, so the logits have to be the sums.
+    Gate rows wider than the matrix, and a routing that only the lower bits decide."""
+    torch, dense, moe = _setup()
+    dt, I = torch.bfloat16, 8
+    w1, w2 = _normal(torch, (experts, I, hidden), dt, 1), _normal(torch, (experts, hidden, I), dt, 2)
+    gate = _whole(torch, (experts, hidden + 3), dt, 3, 9)[:, :hidden]
+    x = _whole(torch, (tokens, hidden), dt, 4, 9)
+    layer = moe.UnquantisedMoeLayer(w1, w1, w2, 2, LIMIT, router_weight_16=gate, score_kind=1)
+    got = layer.router_logits(x)
+    assert got.dtype == torch.float32
+    assert torch.equal(got.double(), _mm64(x, gate))
+    # logits 1 + e / 1024, one step of bf16 at 1 apart at most
+    x = torch.zeros(tokens, hidden, dtype=dt, device="cuda")
+    gate = torch.zeros(experts, hidden, dtype=dt, device="cuda")
+    x[:, 0] = x[:, 1] = 1.0
+    gate[:, 0], gate[:, 1] = 1.0, torch.arange(experts, device="cuda") % 8 / 1024.0
+    layer = moe.UnquantisedMoeLayer(w1, w1, w2, 2, LIMIT, router_weight_16=gate, score_kind=1)
+    _, ids, _ = layer.decode(x)
+    scores = torch.sigmoid(_mm64(x, gate))
+    assert torch.equal(ids.long(), torch.sort(scores, dim=1, descending=True, stable=True).indices[:, :2])

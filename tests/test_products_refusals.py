@@ -200,3 +200,24 @@ def test_a_stack_takes_unquantised_layers_of_fp16_only():
     assert moe.LayerStack([], []).fused is True
     with pytest.raises(ValueError, match="fp16"):
         moe.LayerStack([layer(torch.float16), layer(torch.bfloat16)], [None, None])
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(tokens=-1), "out of range"), (dict(x=None), "null buffer"), (dict(y=None), "null buffer"), (dict(gate=None), "null weight"),
+    (dict(x=ODD), "boundary"), (dict(y=C.c_void_p((1 << 21) + 2)), "boundary"), (dict(gate=ODD), "odd address"),
+    (dict(xs=7167), "row pitch"), (dict(gs=7167), "overlap"), (dict(y=A), "must not alias"), (dict(experts=0), "bad shape"),
+    (dict(ws=None), "workspace of"), (dict(wb=4), "workspace of")])
+def test_bf16_gate_refusals(kw, text):
+    a = dict(x=A, xs=7168, gate=C.c_void_p(1 << 22), gs=7168, y=B, tokens=20, hidden=7168, experts=256, ws=A, wb=1 << 30)
+    a.update(kw)
+    assert capi.lib().aeon_router_logits_bf16_workspace_bytes(20, 7168, 256) > 0
+    with pytest.raises(ValueError, match=text):
+        capi.call("aeon_router_logits_bf16", a["x"], a["xs"], a["gate"], a["gs"], a["y"], a["tokens"], a["hidden"],
+                  a["experts"], a["ws"], a["wb"], None)
+
+
+def test_the_bf16_gate_checks_its_operands():
+    import torch
+    for gate in (torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.float16), torch.zeros(8, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="gate has to be"):
+            dense.router_logits(torch.zeros(2, 8, dtype=torch.bfloat16), gate)
