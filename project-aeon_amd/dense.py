@@ -1,6 +1,7 @@
 """Products over unquantised fp16 / bf16 weights, dense and by expert, over the C ABI: the functions
 take torch tensors on one GPU, run on that GPU's current stream and allocate what they return (and
-the workspace) from torch's allocator, so they can be captured into a graph.
+the workspace) from torch's allocator, so they can be captured into a graph. They have no backward
+pass: where one would be recorded (gradients enabled, an operand that requires one) they refuse.
 
     y   = linear(x, w, bias, activation="gelu", residual=r)
     lists = expert_lists(ids, experts)
@@ -59,6 +60,13 @@ def check_rows(t, name, like, cols):
     if t.dim() != 2:
         raise ValueError("%s has to be a 2-d tensor" % name)
     _check(t, name, like.get_device(), like.dtype, (t.shape[0], cols))
+
+
+def _forward_only(*operands):
+    """A result without a backward pass would drop the operands' gradients and say nothing."""
+    if torch._C._any_requires_grad(*operands) and torch.is_grad_enabled():
+        raise ValueError("an operand requires a gradient, and there is no backward pass: call under torch.no_grad(), or "
+                         "give the operands detached")
 
 
 def _ptr(t):
@@ -124,6 +132,7 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
            residual=None, out=None):
     """act(x @ weight.T + bias) + residual (aeon_linear). x [tokens][in_dim], weight [out_dim][in_dim];
     "swiglu" takes the second matrix as weight_up. `out` may be the residual itself."""
+    _forward_only(x, weight, bias, weight_up, bias_up, residual)
     p = _projection(x, weight, bias, activation, weight_up, bias_up, swiglu_limit, 0)
     device, tokens = x.get_device(), x.shape[0]
     shape = (tokens, p.out_dim)
@@ -141,6 +150,7 @@ def linear(x, weight, bias=None, activation="none", weight_up=None, bias_up=None
 def router_logits(x, gate):
     """fp32 [tokens][experts]: the sums x @ gate.T of a bf16 gate [experts][hidden], unrounded
     (aeon_router_logits_bf16)."""
+    _forward_only(x, gate)
     if gate.dim() != 2 or gate.dtype is not torch.bfloat16 or not gate.is_cuda:
         raise ValueError("gate has to be a 2-d bf16 tensor on a GPU")
     experts, hidden = gate.shape
@@ -188,6 +198,7 @@ def expert_linear(x, weight, offsets, rows=None, bias=None, activation="none", w
     """The same product by expert (aeon_expert_linear): weight [experts][out_dim][in_dim]; expert e's
     positions are offsets[e] .. offsets[e+1]-1, position p takes row rows[p] of x (without `rows`: row p).
     Returns [positions][out_dim]; rows behind the last list are not written."""
+    _forward_only(x, weight, bias, weight_up, bias_up)
     p = _projection(x, weight, bias, activation, weight_up, bias_up, swiglu_limit, 1)
     device, x_rows = x.get_device(), x.shape[0]
     positions = x_rows if rows is None else rows.shape[0]
@@ -203,6 +214,7 @@ def expert_combine(h, weight, offsets, draws, ids, weights, bias=None, base=None
     h [tokens * slots][in_dim] by position, weight [experts][out_dim][in_dim], ids int32 and weights fp32
     [tokens][slots], offsets and draws the lists of these ids: a draw is left out by an id outside
     [0, experts), not by taking it from a list. Returns [tokens][out_dim]; `out` may be the base itself."""
+    _forward_only(h, weight, bias, weights, base)
     p = _projection(h, weight, bias, "none", None, None, 0.0, 1)
     if ids.dim() != 2:
         raise ValueError("ids has to be [tokens][slots]")

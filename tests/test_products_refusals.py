@@ -221,3 +221,32 @@ def test_the_bf16_gate_checks_its_operands():
     for gate in (torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.float16), torch.zeros(8, dtype=torch.bfloat16)):
         with pytest.raises(ValueError, match="gate has to be"):
             dense.router_logits(torch.zeros(2, 8, dtype=torch.bfloat16), gate)
+
+
+def test_nothing_drops_a_gradient_silently():
+    """An operand that requires a gradient is refused while gradients are recorded, whichever it is; without
+    recording, or detached, the call goes on to its other checks (here: no GPU)."""
+    import torch
+    h = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16)
+    lists = torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    ids = torch.zeros(2, 2, dtype=torch.int32)
+    x, y, w, w3, b = h(2, 8), h(4, 8), h(6, 8), h(2, 6, 8), h(6)
+    calls = ((dense.linear, dict(x=x, weight=w, bias=b, weight_up=h(6, 8), bias_up=h(6), residual=h(2, 6), activation="swiglu")),
+             (dense.expert_linear, dict(x=x, weight=w3, offsets=lists[0], rows=lists[1], bias=h(2, 6), weight_up=h(2, 6, 8),
+                                        bias_up=h(2, 6), activation="swiglu")),
+             (dense.expert_combine, dict(h=y, weight=w3, offsets=lists[0], draws=lists[1], ids=ids, weights=torch.zeros(2, 2),
+                                         bias=h(2, 6), base=h(2, 6))),
+             (dense.router_logits, dict(x=x, gate=w)))
+    for call, kw in calls:
+        for name, t in kw.items():
+            if not (isinstance(t, torch.Tensor) and t.is_floating_point()):
+                continue
+            given = dict(kw)
+            given[name] = t.clone().requires_grad_()
+            with pytest.raises(ValueError, match="no backward pass"):
+                call(**given)
+            with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
+                call(**given)
+            given[name] = given[name].detach()
+            with pytest.raises(ValueError, match="on a GPU"):
+                call(**given)
