@@ -156,3 +156,61 @@ def test_logits_of_a_bf16_gate_are_not_rounded(tokens, hidden, experts):
     _, ids, _ = layer.decode(x)
     scores = torch.sigmoid(_mm64(x, gate))
     assert torch.equal(ids.long(), torch.sort(scores, dim=1, descending=True, stable=True).indices[:, :2])
+
+
+def _gated_halves(torch, product, run, dt):
+    """silu(g) * 1 and silu(9) * u of whole-number sums, no clamp: a sum that lacks a term, or has another row's, is
+    off by one at least. fp32 moves the exponential in silu by a few |g| * 2^-24 of itself, and the rest by at
+    most 16 units of 2^-23; half the type's smallest step may be lost, or 2^-120 of fp32's range."""
+    step = torch.finfo(dt).eps / 2
+    least = torch.finfo(dt).smallest_normal * step if dt is torch.float16 else 2.0 ** -120
+    silu9 = 9.0 * torch.special.expit(torch.tensor(9.0, dtype=torch.float64)).item()
+    for up, want, loss in ((False, product * torch.special.expit(product), (4 * product.abs() + 16) * 2.0 ** -23),
+                           (True, product * silu9, 64 * 2.0 ** -23)):
+        got = run(up)
+        loss = want.abs() * loss + least
+        assert not bool(((got.double() - want).abs() > step * (want.abs() + loss) + loss).any())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("tokens,k,n", [(2100, 4168, 4000), (3000, 4104, 2052), (2100, 4167, 4000), (600, 1000, 1030), (70, 1000, 130),
+                                        (3, 512, 48)])
+def test_both_halves_of_a_gated_product(tokens, k, n, dtype):
+    torch, dense, moe = _setup()
+    dt = getattr(torch, dtype)
+    x, w = _whole(torch, (tokens, k), dt, 1, 1), _whole(torch, (n, k), dt, 2, 1)
+    none, flat = torch.zeros_like(w), lambda v: torch.full((n,), v, dtype=dt, device="cuda")
+    print("gated", tokens, k, n, dtype, flush=True)
+
+    def run(up):
+        if up:
+            return dense.linear(x, none, flat(9.0), activation="swiglu", weight_up=w)
+        return dense.linear(x, w, activation="swiglu", weight_up=none, bias_up=flat(1.0))
+
+    product = _mm64(x, w)
+    _gated_halves(torch, product, run, dt)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("tokens,slots,experts,k,n", [(600, 2, 4, 4200, 2080), (300, 6, 24, 264, 1200), (300, 6, 24, 265, 1200),
+                                                      (1, 8, 32, 1024, 96), (64, 4, 16, 520, 130)])
+def test_both_halves_of_a_gated_expert_product(tokens, slots, experts, k, n, dtype):
+    torch, dense, moe = _setup()
+    dt = getattr(torch, dtype)
+    ids = _spread(torch, tokens, slots, experts)
+    lists = dense.expert_lists(ids, experts)
+    x, w = _whole(torch, (tokens, k), dt, 1, 1), _whole(torch, (experts, n, k), dt, 2, 1)
+    none, flat = torch.zeros_like(w), lambda v: torch.full((experts, n), v, dtype=dt, device="cuda")
+    print("gated experts", tokens, slots, experts, k, n, dtype, flush=True)
+
+    def run(up):
+        if up:
+            return dense.expert_linear(x, none, lists.offsets, lists.rows, bias=flat(9.0), activation="swiglu", weight_up=w)
+        return dense.expert_linear(x, w, lists.offsets, lists.rows, activation="swiglu", weight_up=none, bias_up=flat(1.0))
+
+    product = torch.zeros(tokens * slots, n, dtype=torch.float64, device="cuda")
+    bounds = lists.offsets.tolist()
+    for e in range(experts):
+        at = slice(bounds[e], bounds[e + 1])
+        product[at] = _mm64(x[lists.rows[at].long()], w[e])
+    _gated_halves(torch, product, run, dt)
