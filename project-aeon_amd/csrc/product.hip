@@ -112,16 +112,17 @@ __device__ __forceinline__ void activate(int kind, float (&g)[N], const float (&
 // One wave-wide request: 16 bytes of `p` (per lane) to LDS byte `lds` + 16 * lane. Written as
 // asm because the compiler makes every later LDS read wait for all requests of the builtin form.
 // It has no register result, so nothing is in flight that the compiler could reuse; the waits are
-// wait_requests() before the barrier that publishes a stage.
+// wait_requests() before the barrier that publishes a stage. M0 is never live across instructions the
+// compiler emits: it writes it right before each use.
 // STREAM: the bytes are read by this workgroup alone and should not push others out of the caches.
 template <bool STREAM>
 __device__ __forceinline__ void request_to_lds(const char* p, uint32_t lds) {
     if constexpr (STREAM) {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
-                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory", "m0");
+                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
     } else {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory", "m0");
+                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory");
     }
 }
 template <int N>
