@@ -19,8 +19,9 @@
 // What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
 //   4 x any    launch and a trip to memory (1 token, 4096 -> 256: 3.4 us), and the FMAs from two positions on
 //   16..64     the weight stream while it is long: 6.9 TB/s over 12.9 GB (64 tokens, 256 experts); in
-//              short products a workgroup's own start and end, and with 64 positions LDS and the way
-//              from L2 to it (about 80 GB/s a CU)
+//              short products a workgroup's own start and end, and with 64 positions the bytes under way:
+//              half of the ring holds positions (64 tokens, 7168 -> 7168: 224 workgroups ask for 7 MB of
+//              weights ahead, and 103 MB take 24 us)
 //   128, 256   the matrix pipe: a 256 x 256 x 64 step takes 1.36 us where the panels are in L2, 1.58
 //              PFLOP/s; 2.07 us where every weight panel is one workgroup's own and comes from
 //              HBM, because a CU's 64 KB a step then wait for misses of twice the latency
@@ -880,19 +881,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_kernel(const Produ
     else few_body<T, ROWS, MATS, 4>(a, t, sums);
 }
 
-// The weighted sum of a token's expert products in one launch: a workgroup walks the slots of its
-// token for ROWS outputs, so nothing passes through memory between the products and the sum. Every
-// slot streams its expert's rows anew, hence for a few tokens. The slots' chunks of K follow each
-// other in one sequence whose next loads are issued before the present ones are used. At most 64
-// draws: lane l holds draw l's id, weight and position. Measured, us of this kernel / of two launches: 1 and 3 tokens of
-// 8 slots, 2048 -> 7168: 41.8 / 48.6 and 108 / 109; 8 tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.2 / 10.3; 12 tokens
-// (50 MB): 13.5 / 10.3; 4 tokens of 6 slots, 512 -> 2048 (50 MB): 13.3 / 16.5, 6 tokens (75 MB): 19.6 / 18.7. The host
-// spends 4 us less on it.
-// The weight meets a slot's whole product, as in two launches: a weighed part may be infinite, or NaN beside an
-// infinite weight, where the product is neither.
-constexpr int kDirectDraws = 64;
-constexpr int kDirectTokens = 3;
-constexpr double kDirectBytes = 40e6;  // rows streamed, above which more tokens go through memory
 // Sums over the lanes of eight values a lane: of value lane % 8. Three exchanges halve the values a lane holds (with
 // lane ^ 7, ^ 2 and ^ 1, which reach all eight), three steps add what is left over lanes 8, 16 and 32 apart. All of it in
 // the vector pipe, seven moves and three steps: a butterfly through LDS for each value is 48 round trips.
@@ -919,6 +907,18 @@ __device__ __forceinline__ float sum_by_row(const float (&v)[8], int lane) {
     return joined(__builtin_amdgcn_permlane32_swap(bits, bits, false, false));
 }
 
+// The weighted sum of a token's expert products in one launch: a workgroup walks the slots of its
+// token for ROWS outputs, so nothing passes through memory between the products and the sum. Every
+// slot streams its expert's rows anew, hence for a few tokens. The slots' chunks of K follow each
+// other in one sequence whose next loads are issued before the present ones are used. At most 64
+// draws: lane l holds draw l's id, weight and position. The weight meets a slot's whole product, as in two launches: a
+// weighed part may be infinite, or NaN beside an infinite weight, where the product is neither. Measured, us of this
+// kernel / of two launches, cold rows: 1, 3 and 4 tokens of 8 slots, 2048 -> 7168: 41.1 / 46.0, 118 / 121 and 162 / 157; 8
+// tokens of 2 slots, 1024 -> 1024 (34 MB of rows): 9.0 / 12.5; 6 tokens of 6 slots, 512 -> 2048 (75 MB): 18.3 / 20.9. With rows
+// that repeat the two launches were ahead from 50 MB on. The host spends 4 us less on it.
+constexpr int kDirectDraws = 64;
+constexpr int kDirectTokens = 3;
+constexpr double kDirectBytes = 40e6;  // rows streamed, above which more tokens go through memory
 template <class T, int ROWS>
 __global__ __launch_bounds__(64 * kFewWaves) void product_token_kernel(const ProductArgs a, const int32_t* ids, int slots,
                                                                        const uint16_t* base, long base_stride,
@@ -1203,9 +1203,10 @@ struct ProductPlan {
 
 // What a tile costs, us: a 64-column step of a workgroup that has its CU to itself, of one of two that
 // share it (0: it never does), and the rest of a workgroup (launch, first requests, epilogue). Fitted to
-// products of 5 to 4096 tokens with matrices of 1024 x 512 to 14336 x 4096, each at every tile and at one to
-// eight shares, weights cold (120 products; the plan made from these figures is within 0.3 % of the best one
-// measured in the mean, and 7 % at worst).
+// products of 5 to 4096 tokens with matrices of 1024 x 512 to 14336 x 4096, each at every tile of this table and at one
+// to eight shares (120 products; the plan made from these figures is within 0.3 % of the best one measured in the
+// mean, and 7 % at worst). The figures order the tiles; they are not times: a matrix that comes from HBM at every
+// call takes up to 1.6 times its price (128 tokens, 4096 -> 14336: 25.5, measured 40).
 // Without the tiles of 32 rows and the 128 x 128 one that has its CU alone the same products take 6 % more in
 // the mean: 128 tokens, K 2048, N 4096: 12.5 us, 10.7 with 64 x 32; 512 tokens, K = N = 7168: 82, and 69 with 128 x 128.
 struct TileCost {
@@ -1217,8 +1218,10 @@ constexpr TileCost kTileCosts[] = {{kTile32x32, 32, 32, 0.12, 0.29, 2.2}, {kTile
                                    {kTile64x64, 64, 64, 0.19, 0.39, 3.0}, {kTile128Alone, 128, 128, 0.46, 0.0, 8.1},
                                    {kTile256, 256, 256, 1.43, 0.0, 16.0}};
 
-// Every tile and number of shares priced: rounds of workgroups, the weights' way from memory, and the
-// second launch that joins shares with its traffic. The kernel for a few positions pays by eight
+// Each tile of the table priced at 1, 2, 3, 4, 6 and 8 shares: rounds of workgroups, the weights' way from memory
+// (at 9.7 TB/s, what the Infinity Cache gives; HBM 6.7), and the second launch that joins shares with its traffic.
+// The figures are of the kernels for rows on 4-byte boundaries: rows off them take the tile nearest to the planned
+// one that passes through registers, and its shares. The kernel for a few positions pays by eight
 // weight rows: what a workgroup costs beside its loads, more with the FMAs of two or four positions. Measured,
 // us in it / in the best tile: 1 token, 4096 -> 256: 3.4 / 8.5, 7168 -> 7168: 21.1 / 22.6, 512 -> 32000: 18.8 / 9.2;
 // 4 tokens: 4.5 / 8.6, 26.5 / 21.1, 45.6 / 9.3; 8 tokens, 4096 -> 256: 4.7 / 9.0.
