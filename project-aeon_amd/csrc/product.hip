@@ -1206,7 +1206,8 @@ struct ProductPlan {
 // products of 5 to 4096 tokens with matrices of 1024 x 512 to 14336 x 4096, each at every tile of this table and at one
 // to eight shares (120 products; the plan made from these figures is within 0.3 % of the best one measured in the
 // mean, and 7 % at worst). The figures order the tiles; they are not times: a matrix that comes from HBM at every
-// call takes up to 1.6 times its price (128 tokens, 4096 -> 14336: 25.5, measured 40).
+// call takes up to 1.6 times its price (128 tokens, 4096 -> 14336: 25.5, measured 40), and the choice can be off
+// (200 tokens, 7168 -> 28672: 146 us in the planned two shares, 122 in one).
 // Without the tiles of 32 rows and the 128 x 128 one that has its CU alone the same products take 6 % more in
 // the mean: 128 tokens, K 2048, N 4096: 12.5 us, 10.7 with 64 x 32; 512 tokens, K = N = 7168: 82, and 69 with 128 x 128.
 struct TileCost {

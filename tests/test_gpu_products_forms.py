@@ -64,7 +64,7 @@ def _spread(torch, tokens, slots, experts):
 # draws and matrices on both sides of what one launch takes, K with and without a last partial chunk of 512, K of
 # one lane, K of more chunks than waves
 COMBINE_SHAPES = [(1, 8, 16, 1030, 48), (1, 8, 16, 2048, 520), (3, 4, 16, 72, 130), (2, 1, 5, 8, 9), (8, 2, 7, 4104, 24),
-                  (1, 3, 5, 7, 16), (20, 4, 16, 1030, 48), (40, 2, 16, 520, 130)]
+                  (1, 3, 5, 7, 16), (1, 64, 80, 520, 24), (2, 32, 7, 1030, 9), (20, 4, 16, 1030, 48), (40, 2, 16, 520, 130)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
@@ -115,6 +115,17 @@ def test_combine_weighs_the_product_and_not_its_parts(tokens, k):
     assert bool((out.double() == 2.0 ** 122).all())
 
 
+@pytest.mark.parametrize("tokens,hidden,experts", [(2100, 4168, 8000), (2100, 4167, 8000), (128, 7168, 1024), (1, 4096, 4096),
+                                                   (9000, 72, 256), (0, 64, 8), (4, 64, 1)])
+def test_logits_of_any_size(tokens, hidden, experts):
+    """dense.router_logits alone, uncut products on the largest tiles among them, into memory that ends with them."""
+    torch, dense, moe = _setup()
+    x, gate = _whole(torch, (tokens, hidden), torch.bfloat16, 1, 9), _whole(torch, (experts, hidden), torch.bfloat16, 2, 9)
+    print("logits", tokens, hidden, experts, flush=True)
+    got = dense.router_logits(x, gate)
+    assert got.shape == (tokens, experts) and torch.equal(got.double(), _mm64(x, gate))
+
+
 def test_a_stack_of_unquantised_layers_as_it_defaults():
     """LayerStack(layers, mixes) with nothing else said: the bits of the stack without the fused tail."""
     torch, dense, moe = _setup()
@@ -131,6 +142,11 @@ def test_a_stack_of_unquantised_layers_as_it_defaults():
     got = moe.LayerStack(layers, mixes).step(residual.clone())
     want = moe.LayerStack(layers, mixes, fused=False).step(residual.clone())
     assert torch.equal(got, want) and bool(got.isfinite().all())
+    # buffers that every layer reuses, twice: nothing of an earlier step stays in them
+    scratch = (torch.empty_like(residual), torch.empty_like(residual[0]), torch.empty_like(residual[0]),
+               torch.empty(tokens, k, dtype=torch.int32, device="cuda"), torch.empty(tokens, k, device="cuda"))
+    for _ in range(2):
+        assert torch.equal(moe.LayerStack(layers, mixes).step(residual.clone(), scratch=scratch), want)
 
 
 @pytest.mark.parametrize("tokens,hidden,experts", [(1, 4096, 256), (1, 100, 7), (3, 512, 24), (20, 7168, 256), (33, 520, 40),
