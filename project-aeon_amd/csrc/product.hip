@@ -18,7 +18,7 @@
 //
 // What bounds it, by tile (positions x rows; chosen by plan_linear and plan_experts):
 //   4 x any    launch and a trip to memory (1 token, 4096 -> 256: 3.4 us), and the FMAs from two positions on
-//   16..64     the weight stream while it is long: 6.9 TB/s over 12.9 GB (64 tokens, 256 experts); in
+//   16..64     the weight stream while it is long: 7.1 TB/s over 12.9 GB (64 tokens, 256 experts); in
 //              short products a workgroup's own start and end, and with 64 positions the bytes under way:
 //              half of the ring holds positions (64 tokens, 7168 -> 7168: 224 workgroups ask for 7 MB of
 //              weights ahead, and 103 MB take 24 us)
